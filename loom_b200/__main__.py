@@ -11,6 +11,10 @@
                                 [--disable-opt FLAG ...]
     python -m loom_b200 list-entries FILE [--input-kind python]
     python -m loom_b200 front-ir FILE --entry E [--input-kind python]
+    python -m loom_b200 train-ops --out OUT [--kind shared|static]
+
+``train-ops`` has no counterpart in ``loomc``: it builds the training-step
+operator package (``train_package.py``).
 
 Entries are read from ``*.tensor_ir.json`` files (the TensorIR the reference
 front end dumps with ``--emit tensor-ir``), from ``*.front_ir.json`` files
@@ -25,7 +29,7 @@ from __future__ import annotations
 import argparse
 import sys
 
-from . import artifact
+from . import artifact, train_package
 from .frontend import FrontendError
 from .optconfig import DEFAULT_CONFIG, OptionsError, load_config, parse_cli_flags
 from .tensor_ir import TensorIRError
@@ -135,8 +139,15 @@ def main(argv=None) -> int:
     fi.add_argument("--entry", required=True)
     fi.add_argument("--input-kind", default="auto")
 
+    to = sub.add_parser("train-ops", help="build the training-step operator package")
+    to.add_argument("--out", required=True)
+    to.add_argument("--kind", default="shared", choices=["shared", "static"])
+
     ns = ap.parse_args(argv)
     try:
+        if ns.cmd == "train-ops":
+            print(train_package.generate_train_package(ns.out, ns.kind).artifact_path)
+            return 0
         if ns.cmd == "list-entries":
             return list_entries(ns.file, _input_kind(ns.input_kind))
         if ns.cmd == "front-ir":

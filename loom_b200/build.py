@@ -4,7 +4,8 @@
 configurations of the hot path, module ``kernels``) into
 ``loom_b200/_built/b200_suite/`` with the reference's default flags (so the
 plain entry points synchronise like the reference's); ``load_suite()`` loads
-it.  The built ``.so`` stays in the tree so that it travels with the
+it.  ``build_train()`` and ``load_train()`` do the same for the training-step
+operators.  The built ``.so`` stays in the tree so that it travels with the
 repository to the GPU machine.
 """
 
@@ -12,13 +13,15 @@ from __future__ import annotations
 
 import os
 
-from . import artifact
+from . import artifact, train_package
 from .loader import Package
+from .train_ops import TrainPackage
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SUITE_PROJECT = os.path.join(HERE, "suite")
 BUILT_DIR = os.path.join(HERE, "_built")
 SUITE_DIR = os.path.join(BUILT_DIR, "b200_suite")
+TRAIN_DIR = os.path.join(BUILT_DIR, train_package.PACKAGE)
 
 
 # Reference flags that change how map bodies are rendered; the body-coverage
@@ -83,6 +86,23 @@ def load_suite() -> Package:
             f"{lib} is missing: build it with `python -c 'import loom_b200.build as b; "
             "b.build_suite()'` (needs nvcc)")
     return Package(SUITE_DIR)
+
+
+def build_train(force: bool = False) -> artifact.PackageResult:
+    lib = os.path.join(TRAIN_DIR, f"lib{train_package.PACKAGE}.so")
+    newest = max(_newest_source_mtime(), os.path.getmtime(train_package.HEADER))
+    if not force and os.path.exists(lib) and os.path.getmtime(lib) >= newest:
+        return None
+    return train_package.generate_train_package(TRAIN_DIR)
+
+
+def load_train() -> TrainPackage:
+    lib = os.path.join(TRAIN_DIR, f"lib{train_package.PACKAGE}.so")
+    if not os.path.exists(lib):
+        raise FileNotFoundError(
+            f"{lib} is missing: build it with `python -c 'import loom_b200.build as b; "
+            "b.build_train()'` (needs nvcc)")
+    return TrainPackage(TRAIN_DIR)
 
 
 def build_project(project_dir: str, force: bool = False, enabled=(), name: str = None) -> str:

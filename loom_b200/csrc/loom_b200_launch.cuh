@@ -183,6 +183,28 @@ inline void launch_pdl(Kern kernel, unsigned grid, cudaStream_t stream, Args... 
   kernel<<<grid, kThreads, 0, stream>>>(args...);
 }
 
+// The same launch with any grid and block; returns a status.
+template <class Kern, class... Args>
+inline int launch_dependent(Kern kernel, dim3 grid, dim3 block, cudaStream_t stream,
+                            const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return LOOM_STATUS_OK;
+  cudaGetLastError();
+  cfg.numAttrs = 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return LOOM_STATUS_OK;
+  cudaGetLastError();
+  return LOOM_STATUS_CUDA_ERROR;
+}
+
 inline unsigned clamp_grid(int64_t g, int64_t cap) {
   if (g > cap) g = cap;
   if (g < 1) g = 1;
