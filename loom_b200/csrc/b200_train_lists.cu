@@ -108,6 +108,8 @@ int adamw_impl(const AdamLists& l, int param_dtype, int grad_dtype, const float*
   c.beta2 = (float)beta2;
   c.rest2 = (float)(1.0 - beta2);
   c.eps = (float)eps;
+  c.zero = -0.0f;
+  c.sixteen = 16u;
   StepValues* values = reinterpret_cast<StepValues*>(loomb::workspace_base(workspace));
   const int st = loomb::launch_dependent(loomb::adamw_begin_kernel, dim3(1), dim3(32), stream,
                                          values, lr, grad_scale, step, beta1, beta2, seed);

@@ -18,10 +18,14 @@
 namespace loomb {
 
 // Largest number of tensors per launch: a table fits the 32764 bytes of a
-// kernel's parameters.  Longer lists take several launches.
+// kernel's parameters.  Longer lists take several launches; lists of at most
+// kShortCap tensors take a table of that size, since a launch costs the more the
+// more parameters it has (a step of six tensors: 5.8 against 7.5 us).
+constexpr int kShortCap = 32;
 constexpr int kNormCap = 1024;
 constexpr int kAdamCap = 480;
 constexpr int kAdam8Cap = 360;
+constexpr int kSms = 148;                // of a B200
 
 // What a kernel's parameters may take beside its table.
 constexpr size_t kParamBytes = 32764, kOtherParams = 256;
@@ -51,10 +55,15 @@ struct NormTile {
   static constexpr int value = kThreads * kNormUnroll * (16 / (int)sizeof(T));
 };
 
+struct NormItem {
+  const void* g;
+  int64_t n;
+};
+
+template <int kCap>
 struct NormTable {
-  const void* g[kNormCap];
-  int64_t n[kNormCap];
-  uint32_t first[kNormCap];
+  NormItem item[kCap];
+  uint32_t first[kCap];
   int count;
   uint32_t tiles;
 };
@@ -64,17 +73,17 @@ struct NormTable {
 // squares of a tile in fp32 (a fixed tree: no cancellation, at most 5
 // roundings, 3e-7 of the tile's sum) and everything past that in fp64.  A
 // square beyond the fp32 range makes the sum infinite.
-template <class T>
+template <class T, int kCap>
 __global__ void __launch_bounds__(kThreads)
-list_norm_kernel(const __grid_constant__ NormTable t, double* __restrict__ partials) {
+list_norm_kernel(const __grid_constant__ NormTable<kCap> t, double* __restrict__ partials) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
   constexpr int V = 16 / (int)sizeof(T);
   double acc = 0.0;
   for (uint32_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
     const int i = find_tensor(t.first, t.count, tile);
-    const T* __restrict__ g = static_cast<const T*>(t.g[i]);
-    const int64_t n = t.n[i];
+    const T* __restrict__ g = static_cast<const T*>(t.item[i].g);
+    const int64_t n = t.item[i].n;
     // elements before the first 16-byte boundary, and whole vectors after it
     const int64_t lead = (int64_t)((16u - ((uintptr_t)g & 15u)) & 15u) / (int)sizeof(T);
     const int64_t head = lead < n ? lead : n;
@@ -128,7 +137,7 @@ list_norm_kernel(const __grid_constant__ NormTable t, double* __restrict__ parti
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
-static_assert(sizeof(NormTable) + kOtherParams <= kParamBytes, "the list fits the parameters");
+static_assert(sizeof(NormTable<kNormCap>) + kOtherParams <= kParamBytes, "the list fits the parameters");
 
 // out[0] = the norm, out[1] = the factor that brings it down to max_norm: 1
 // where it is no larger, NaN where the sum is not finite (a step given that
@@ -157,22 +166,21 @@ inline size_t list_norm_workspace_bytes(int64_t count) {
   return (size_t)list_launches(count, kNormCap) * kNormMaxCtas * sizeof(double) + 256;
 }
 
-template <class T>
-inline int launch_list_norm(int64_t count, const void* const* grads, const int64_t* sizes,
+template <class T, int kCap>
+inline int launch_list_norm_parts(int64_t count, const void* const* grads, const int64_t* sizes,
                             float max_norm, float* out, void* workspace, cudaStream_t stream) {
   double* partials = reinterpret_cast<double*>(workspace_base(workspace));
   int filled = 0;
-  NormTable t;
+  NormTable<kCap> t;
   int64_t i = 0;
   while (i < count) {
     t.count = 0;
     int64_t tiles = 0;
-    for (; i < count && t.count < kNormCap; ++i) {
+    for (; i < count && t.count < kCap; ++i) {
       if (sizes[i] == 0) continue;
       const int64_t more = ceil_div(sizes[i], (int64_t)NormTile<T>::value);
       if (tiles + more > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
-      t.g[t.count] = grads[i];
-      t.n[t.count] = sizes[i];
+      t.item[t.count] = {grads[i], sizes[i]};
       t.first[t.count] = (uint32_t)tiles;
       ++t.count;
       tiles += more;
@@ -180,7 +188,7 @@ inline int launch_list_norm(int64_t count, const void* const* grads, const int64
     if (t.count == 0) break;
     t.tiles = (uint32_t)tiles;
     const unsigned grid = clamp_grid(tiles, kNormMaxCtas);
-    const int st = launch_dependent(list_norm_kernel<T>, dim3(grid), dim3(kThreads),
+    const int st = launch_dependent(list_norm_kernel<T, kCap>, dim3(grid), dim3(kThreads),
                                     stream, t, partials + filled);
     if (st != LOOM_STATUS_OK) return st;
     filled += (int)grid;
@@ -193,13 +201,14 @@ inline int launch_list_norm(int64_t count, const void* const* grads, const int64
 // AdamW
 
 // What a step computes once: left in the workspace by adamw_begin_kernel.
-struct StepValues {
+struct alignas(16) StepValues {
   float scale;    // gradient factor
   float rate;     // lr / (1 - beta1^t)
   float root;     // 1 / sqrt(1 - beta2^t)
   float lr;
   uint32_t key;   // of this step's random numbers
   uint32_t skip;  // the factor is not finite: nothing is changed
+  uint32_t unused[2];
 };
 
 // The constants of a step, rounded once on the host from fp64.
@@ -207,6 +216,8 @@ struct StepConst {
   float beta1, rest1;  // beta, 1 - beta
   float beta2, rest2;
   float eps;
+  float zero;           // -0, added to a product that must be rounded on its own
+  uint32_t sixteen;     // 16, for a shift on the multiplier
 };
 
 // A bijection of 32-bit words in which each input bit moves about half of the
@@ -229,7 +240,7 @@ __global__ void adamw_begin_kernel(StepValues* __restrict__ out, const float* __
   allow_dependent_launch();
   wait_for_prerequisite_grid();
   if (threadIdx.x != 0) return;
-  StepValues s;
+  StepValues s = {};
   s.scale = grad_scale != nullptr ? *grad_scale : 1.0f;
   s.skip = !(fabsf(s.scale) < INFINITY);
   const int64_t t = *step + (s.skip ? 0 : 1);
@@ -246,14 +257,20 @@ __global__ void adamw_begin_kernel(StepValues* __restrict__ out, const float* __
 
 inline size_t adamw_workspace_bytes() { return 256 + 256; }
 
+// Plain loads, which stay in an SM's first-level cache: every warp of the grid
+// reads these 32 bytes, and asking the second level for them each time made
+// its one line the whole step's limit (1026 us for 109M fp32 parameters in
+// tiles of 1024, against 466 for their bytes).  The wait at the kernel's start
+// makes what the kernel before it wrote visible to them.
 __device__ __forceinline__ StepValues step_values(const StepValues* p) {
+  const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
   StepValues s;
-  s.scale = __ldcg(&p->scale);
-  s.rate = __ldcg(&p->rate);
-  s.root = __ldcg(&p->root);
-  s.lr = __ldcg(&p->lr);
-  s.key = __ldcg(&p->key);
-  s.skip = __ldcg(&p->skip);
+  s.scale = __uint_as_float(a.x);
+  s.rate = __uint_as_float(a.y);
+  s.root = __uint_as_float(a.z);
+  s.lr = __uint_as_float(a.w);
+  s.key = b.x;
+  s.skip = b.y;
   return s;
 }
 
@@ -273,18 +290,22 @@ __device__ __forceinline__ float stepped(float p, float m, float v, const StepCo
   return p * keep - s.rate * move;
 }
 
-constexpr int kAdamUnroll = 2;                           // groups of four elements per thread
-constexpr int kAdamTile = kThreads * 4 * kAdamUnroll;    // elements per CTA
+constexpr int kAdamTile = kThreads * 4;                  // elements per CTA
 
+struct AdamItem {
+  void* p;
+  const void* g;
+  float* m;
+  float* v;
+  float* w;                   // fp32 master copy (unused without them)
+  int64_t n;
+  double decay;
+};
+
+template <int kCap>
 struct AdamTable {
-  void* p[kAdamCap];
-  const void* g[kAdamCap];
-  float* m[kAdamCap];
-  float* v[kAdamCap];
-  float* w[kAdamCap];         // fp32 master copies (unused without them)
-  int64_t n[kAdamCap];
-  double decay[kAdamCap];
-  uint32_t first[kAdamCap];
+  AdamItem item[kCap];
+  uint32_t first[kCap];
   int count;
 };
 
@@ -294,25 +315,27 @@ __device__ __forceinline__ unsigned phase4(const T* p) {
 }
 
 // HBM-bound: 28 bytes and about 14 operations an element with fp32 parameters
-// or with fp32 masters.  Four consecutive elements per access (16 bytes of
-// every fp32 array); where the arrays of a tensor stand at different places
-// mod 4 elements, single elements are moved instead.
-template <class Tp, class Tg, bool kMaster>
-__global__ void __launch_bounds__(kThreads)
-adamw_kernel(const __grid_constant__ AdamTable t, const StepValues* __restrict__ values,
+// or with fp32 masters; 109M fp32 parameters take 442 us, 105% of the copy
+// rate.  Four consecutive elements per thread (16 bytes of every fp32 array)
+// and six CTAs per SM: eight or sixteen elements a thread leave fewer warps to
+// cover the loads' latency (455 and 453 us).  Where the arrays of a tensor stand
+// at different places mod 4 elements, single elements are moved instead.
+template <class Tp, class Tg, bool kMaster, int kCap>
+__global__ void __launch_bounds__(kThreads, 6)
+adamw_kernel(const __grid_constant__ AdamTable<kCap> t, const StepValues* __restrict__ values,
              const StepConst c) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
   const int i = find_tensor(t.first, t.count, blockIdx.x);
   const StepValues s = step_values(values);
-  if (s.skip) return;
-  Tp* const p = static_cast<Tp*>(t.p[i]);
-  const Tg* const g = static_cast<const Tg*>(t.g[i]);
-  float* const m = t.m[i];
-  float* const v = t.v[i];
-  float* const w = kMaster ? t.w[i] : nullptr;
-  const int64_t n = t.n[i];
-  const float keep = (float)(1.0 - (double)s.lr * t.decay[i]);
+  const AdamItem& item = t.item[i];
+  Tp* const p = static_cast<Tp*>(item.p);
+  const Tg* const g = static_cast<const Tg*>(item.g);
+  float* const m = item.m;
+  float* const v = item.v;
+  float* const w = kMaster ? item.w : nullptr;
+  const int64_t n = item.n;
+  const float keep = (float)(1.0 - (double)s.lr * item.decay);
   const int64_t tile = blockIdx.x - t.first[i];
 
   auto one = [&](int64_t e) {
@@ -330,8 +353,9 @@ adamw_kernel(const __grid_constant__ AdamTable t, const StepValues* __restrict__
   const bool together = phase4(v) == ph && phase4(p) == ph && phase4(g) == ph &&
                         (!kMaster || phase4(w) == ph);
   if (!together) {
+    if (s.skip) return;
 #pragma unroll 1
-    for (int u = 0; u < 4 * kAdamUnroll; ++u) {
+    for (int u = 0; u < 4; ++u) {
       const int64_t e = tile * kAdamTile + u * kThreads + threadIdx.x;
       if (e < n) one(e);
     }
@@ -340,38 +364,30 @@ adamw_kernel(const __grid_constant__ AdamTable t, const StepValues* __restrict__
   const int64_t lead = (4u - ph) & 3u;
   const int64_t head = lead < n ? lead : n;
   const int64_t nvec = (n - head) >> 2;
-  const int64_t v0 = tile * (kThreads * kAdamUnroll) + threadIdx.x;
-  float fp[kAdamUnroll][4], fg[kAdamUnroll][4], fm[kAdamUnroll][4], fv[kAdamUnroll][4];
-#pragma unroll
-  for (int u = 0; u < kAdamUnroll; ++u) {
-    const int64_t at = v0 + u * kThreads;
-    if (at < nvec) {
-      const int64_t e = head + at * 4;
-      if (kMaster) {
-        load_vec<4, kStream>(fp[u], (const float*)w + e);
-      } else {
-        load_vec<4, kStream>(fp[u], (const Tp*)p + e);
-      }
-      load_vec<4, kStream>(fg[u], g + e);
-      load_vec<4, kStream>(fm[u], (const float*)m + e);
-      load_vec<4, kStream>(fv[u], (const float*)v + e);
+  const int64_t at = tile * kThreads + threadIdx.x;
+  const int64_t e = head + at * 4;
+  float fp[4], fg[4], fm[4], fv[4];
+  if (at < nvec) {
+    if (kMaster) {
+      load_vec<4, kStream>(fp, (const float*)w + e);
+    } else {
+      load_vec<4, kStream>(fp, (const Tp*)p + e);
     }
+    load_vec<4, kStream>(fg, g + e);
+    load_vec<4, kStream>(fm, (const float*)m + e);
+    load_vec<4, kStream>(fv, (const float*)v + e);
   }
+  if (s.skip) return;  // looked at when the data is on its way
+  if (at < nvec) {
 #pragma unroll
-  for (int u = 0; u < kAdamUnroll; ++u) {
-    const int64_t at = v0 + u * kThreads;
-    if (at < nvec) {
-      const int64_t e = head + at * 4;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        moments(fm[u][j], fv[u][j], fg[u][j], c, s.scale);
-        fp[u][j] = stepped(fp[u][j], fm[u][j], fv[u][j], c, s, keep);
-      }
-      store_vec<4, kStream>(m + e, fm[u]);
-      store_vec<4, kStream>(v + e, fv[u]);
-      if (kMaster) store_vec<4, kStream>(w + e, fp[u]);
-      store_vec<4, kStream>(p + e, fp[u]);
+    for (int j = 0; j < 4; ++j) {
+      moments(fm[j], fv[j], fg[j], c, s.scale);
+      fp[j] = stepped(fp[j], fm[j], fv[j], c, s, keep);
     }
+    store_vec<4, kStream>(m + e, fm);
+    store_vec<4, kStream>(v + e, fv);
+    if (kMaster) store_vec<4, kStream>(w + e, fp);
+    store_vec<4, kStream>(p + e, fp);
   }
   if (tile == 0) {  // the tensor's first tile takes its ragged ends
     const int64_t tail0 = head + (nvec << 2);
@@ -385,184 +401,402 @@ adamw_kernel(const __grid_constant__ AdamTable t, const StepValues* __restrict__
 // AdamW with 8-bit states
 
 constexpr int kBlock = 256;                              // values that share one top
-constexpr int kTileBlocks = kThreads / 32;               // one block per warp
+constexpr int kMaxWarpBlocks = 16;                       // consecutive blocks per warp
 constexpr float kTop = 256.0f;                           // code value of a block's largest
 constexpr float kTinyTop = 7.8886090522101181e-31f;      // 2^-100: smaller blocks hold zeros
 
+struct Adam8Item {
+  void* p;
+  const void* g;
+  uint8_t* m;
+  uint8_t* v;
+  float* mtop;
+  float* vtop;
+  float* w;
+  int64_t n;
+  double decay;
+  uint64_t block;              // first block, counted through the whole list
+};
+
+template <int kCap>
 struct Adam8Table {
-  void* p[kAdam8Cap];
-  const void* g[kAdam8Cap];
-  uint8_t* m[kAdam8Cap];
-  uint8_t* v[kAdam8Cap];
-  float* mtop[kAdam8Cap];
-  float* vtop[kAdam8Cap];
-  float* w[kAdam8Cap];
-  int64_t n[kAdam8Cap];
-  double decay[kAdam8Cap];
-  uint32_t first[kAdam8Cap];   // first tile
-  uint32_t block[kAdam8Cap];   // first block, counted through the whole list
+  Adam8Item item[kCap];
+  uint32_t first[kCap];   // first tile
   int count;
+  int warp_blocks;             // consecutive blocks that each warp takes
+};
+
+// Eight consecutive elements as they lie in memory.
+template <class T>
+struct Raw8 {
+  uint4 word[sizeof(T) / 2];
 };
 
 // Eight consecutive elements of which the first `left` exist; the others are
-// zero.  `whole`: p is aligned for one vector access.
+// zero.
 template <class T>
-__device__ __forceinline__ void load8(float (&f)[8], const T* p, int left, bool whole) {
-  if (whole && left >= 8) {
-    load_vec<8, kStream>(f, p);
-    return;
+__device__ __forceinline__ void load8_some(Raw8<T>& r, const T* p, int left) {
+  using Bits = typename Word<sizeof(T)>::T;
+  const Bits* q = reinterpret_cast<const Bits*>(p);
+  unsigned u[2 * sizeof(T)];
+#pragma unroll
+  for (int k = 0; k < 2 * (int)sizeof(T); ++k) {
+    if constexpr (sizeof(T) == 4) {
+      u[k] = k < left ? q[k] : 0u;
+    } else {
+      u[k] = (2 * k < left ? q[2 * k] : 0u) | (2 * k + 1 < left ? q[2 * k + 1] : 0u) << 16;
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = j < left ? widen(p[j]) : 0.0f;
+  for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+    r.word[k] = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8], int left, bool whole) {
-  if (whole && left >= 8) {
-    store_vec<8, kStream>(p, f);
-    return;
+__device__ __forceinline__ F2 pair_of(const Raw8<T>& r, int j) {
+  const unsigned* u = reinterpret_cast<const unsigned*>(r.word);
+  if constexpr (sizeof(T) == 4) {
+    return f2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+  } else {
+    float a, b;
+    widen2(a, b, u[j], T());
+    return f2(a, b);
   }
+}
+template <class T>
+__device__ __forceinline__ void store8_some(T* p, const float (&f)[8], int left) {
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (j < left) p[j] = narrow<T>(f[j]);
 }
-__device__ __forceinline__ uint2 load8_codes(const uint8_t* p, int left, bool whole) {
-  if (whole && left >= 8) return __ldcs(reinterpret_cast<const uint2*>(p));
+__device__ __forceinline__ uint2 load8_codes_some(const uint8_t* p, int left) {
   uint2 w = make_uint2(0, 0);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (j < left) (j < 4 ? w.x : w.y) |= (unsigned)p[j] << (8 * (j & 3));
   return w;
 }
-__device__ __forceinline__ void store8_codes(uint8_t* p, uint2 w, int left, bool whole) {
-  if (whole && left >= 8) {
-    __stcs(reinterpret_cast<uint2*>(p), w);
-    return;
-  }
+__device__ __forceinline__ void store8_codes_some(uint8_t* p, uint2 w, int left) {
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (j < left) p[j] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
 }
 
-// Two e4m3 codes (the low 16 bits of `pair`) as fp32.
-__device__ __forceinline__ float2 open2(unsigned pair) {
-  unsigned h;
-  asm("{.reg .b16 c; cvt.u16.u32 c, %1; cvt.rn.f16x2.e4m3x2 %0, c;}" : "=r"(h) : "r"(pair));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-__device__ __forceinline__ void open8(float (&f)[8], uint2 w, float unit) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const unsigned word = j < 2 ? w.x : w.y;
-    const float2 a = open2((j & 1) ? word >> 16 : word);
-    f[2 * j] = __fmul_rn(a.x, unit);
-    f[2 * j + 1] = __fmul_rn(a.y, unit);
-  }
-}
-
-// The e4m3 code of a >= 0 (a <= 256 and a little), rounded up with the
-// probability of its distance from the code below, by the 20-bit number r.
-// A code keeps 3 bits after the leading one: the upper 12 bits of the fp32
-// word, after adding r to the 20 that are cut off.  Below 2^-6 codes are
-// evenly spaced; adding 2^-6 moves that range onto the spacing above it.
-__device__ __forceinline__ unsigned close1(float a, unsigned r) {
-  const bool low = a < 0.015625f;
-  const unsigned bits = __float_as_uint(__fadd_rn(a, low ? 0.015625f : 0.0f)) + r;
-  return (bits >> 20) - (low ? (120u << 3) + 8u : (120u << 3));
+// Four e4m3 codes as fp32.
+__device__ __forceinline__ void open4(F2& lo, F2& hi, unsigned codes) {
+  unsigned a, b;
+  asm("{.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;}"
+      : "=r"(a), "=r"(b)
+      : "r"(codes));
+  const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  lo = f2(fa.x, fa.y);
+  hi = f2(fb.x, fb.y);
 }
 
-// HBM-bound by its bytes (10 and a sixteenth an element with bf16 parameters
-// and gradients), and close to bound by issue: about 75 instructions an
-// element for opening and closing two codes, the random bits and the step.
-// A warp holds one block, eight consecutive values a lane, so a block's
-// largest is one warp-wide maximum of the values' bit patterns; as unsigned
-// words these order NaN above infinity above every number, so a block that
-// holds one that is not finite gets it as its top and reads back as such.
-template <class Tp, class Tg, bool kMaster>
-__global__ void __launch_bounds__(kThreads)
-adamw8_kernel(const __grid_constant__ Adam8Table t, const StepValues* __restrict__ values,
+// Rounds a >= 0 (a <= 256 and a little) to an e4m3 code, up with the
+// probability of its distance from the code below, by the 16 random bits r.
+// A code keeps 3 bits after the leading one, so it is the upper 12 bits of
+// the fp32 word, less the difference of the exponents' offsets (120 << 3),
+// after adding the 20 random bits (r << 4 | 8) to those that are cut off.
+// Below 2^-6 codes are evenly spaced: adding 2^-6 to the value (`lifted`)
+// moves that range onto the binade above it, whose spacing it has, and
+// subtracting a binade from the word moves it back.  The fp32 word as a
+// function of the value is concave, so the lifted word is the larger of the
+// two below 2^-6 and the smaller above, and no comparison of a is needed.
+__device__ __forceinline__ int rounding_word(float a, float lifted) {
+  return __viaddmax_s32(__float_as_int(lifted), -(1 << 23), __float_as_int(a));
+}
+constexpr int kCodeOffset = 960 << 20;
+// The code in the upper byte: word + 8 - offset, moved up by 4.  Written as a
+// product with a kernel argument, the shift goes to the multiplier: the integer
+// pipe is the busiest one here (226 against 229 us for 109M bf16 parameters;
+// moving the random bits' shifts as well made it 233).
+__device__ __forceinline__ unsigned upper_code(int word, unsigned sixteen) {
+  return (unsigned)word * sixteen + ((unsigned)(8 - kCodeOffset) << 4);
+}
+
+// Rates of two and one instructions for the parameter's move, which hangs on
+// no border: about 2 ulp each.
+__device__ __forceinline__ float root_approx(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float inverse_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float largest(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// One lane's part of a block on its way through shared memory.  A lane copies
+// what it reads itself (cp.async), so that its own wait is all that is needed
+// between the two.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(to)),
+               "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copy8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(to)),
+               "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLater>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory");
+}
+
+template <class Tw, class Tg>
+struct BlockStage {
+  uint4 w[sizeof(Tw) / 2][kThreads];
+  uint4 g[sizeof(Tg) / 2][kThreads];
+  uint2 m[kThreads];
+  uint2 v[kThreads];
+};
+
+// 10 and a sixteenth bytes an element with bf16 parameters and gradients, but
+// bound by issue before HBM: about 60 instructions an element for opening and
+// closing two codes, the random bits and the step.  109M bf16 parameters take
+// 226 us, 74% of the copy rate (one block per warp, 115 instructions an element
+// and loads that nothing overlapped: 587 us).  What it rests on:
+//  * a warp holds a block, eight consecutive values a lane, so a block's
+//    largest is one warp-wide maximum of the values' bit patterns; as unsigned
+//    words these order NaN above infinity above every number, so a block that
+//    holds one that is not finite gets it as its top and reads back as such;
+//  * a warp walks up to 16 consecutive blocks; whole blocks come through shared
+//    memory, three (two for wider types) ahead, at no registers' cost;
+//  * packed fp32 instructions for two values at a time;
+//  * three CTAs per SM: bounding the registers for four spills them and is 8%
+//    slower.
+template <class Tp, class Tg, bool kMaster, int kCap>
+__global__ void __launch_bounds__(kThreads, 3)
+adamw8_kernel(const __grid_constant__ Adam8Table<kCap> t, const StepValues* __restrict__ values,
               const StepConst c) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
+  using Tw = typename std::conditional<kMaster, float, Tp>::type;  // what the step reads
   const int i = find_tensor(t.first, t.count, blockIdx.x);
-  const StepValues s = step_values(values);
-  if (s.skip) return;
+  const Adam8Item& item = t.item[i];
   const int lane = threadIdx.x & 31;
-  const int64_t block = (int64_t)(blockIdx.x - t.first[i]) * kTileBlocks + (threadIdx.x >> 5);
-  const int64_t n = t.n[i];
-  if (block * kBlock >= n) return;
-  const int64_t e = block * kBlock + lane * 8;
-  const int left = (int)(n - e < 0 ? 0 : n - e > 8 ? 8 : n - e);
-  Tp* const p = static_cast<Tp*>(t.p[i]);
-  const Tg* const g = static_cast<const Tg*>(t.g[i]);
-  uint8_t* const m = t.m[i];
-  uint8_t* const v = t.v[i];
-  float* const w = kMaster ? t.w[i] : nullptr;
-  const bool p_whole = ((uintptr_t)p & 15u) == 0, g_whole = ((uintptr_t)g & 15u) == 0;
-  const bool m_whole = ((uintptr_t)m & 7u) == 0, v_whole = ((uintptr_t)v & 7u) == 0;
-  const bool w_whole = ((uintptr_t)w & 15u) == 0;
+  const int blocks = t.warp_blocks;
+  const int64_t block =
+      ((int64_t)(blockIdx.x - t.first[i]) * (kThreads / 32) + (threadIdx.x >> 5)) * blocks;
+  const int64_t rest = item.n - block * kBlock;  // elements from the warp's first on
+  const int64_t at = block * kBlock + lane * 8;
+  Tp* p = static_cast<Tp*>(item.p) + at;
+  Tw* w = (kMaster ? (Tw*)item.w : (Tw*)item.p) + at;
+  const Tg* g = static_cast<const Tg*>(item.g) + at;
+  uint8_t* m = item.m + at;
+  uint8_t* v = item.v + at;
+  const bool aligned = (((uintptr_t)p | (uintptr_t)w | (uintptr_t)g) & 15u) == 0 &&
+                       (((uintptr_t)m | (uintptr_t)v) & 7u) == 0;
+  // the warp's blocks, and those of them that lie wholly in the tensor (none
+  // where an array is not aligned for vector access)
+  const int here = rest <= 0 ? 0 : (int)min((rest + kBlock - 1) / kBlock, (int64_t)blocks);
+  const int whole = aligned && rest > 0 ? (int)min(rest / kBlock, (int64_t)blocks) : 0;
+  uint32_t count = (uint32_t)(item.block + block) * 32u + lane;
 
-  float fp[8], fg[8], fm[8], fv[8];
-  if (kMaster) {
-    load8(fp, (const float*)w + e, left, w_whole);
-  } else {
-    load8(fp, (const Tp*)p + e, left, p_whole);
-  }
-  load8(fg, g + e, left, g_whole);
-  const uint2 mc = load8_codes(m + e, left, m_whole);
-  const uint2 vc = load8_codes(v + e, left, v_whole);
-  const float mt = t.mtop[i][block], vt = t.vtop[i][block];
-  const float keep = (float)(1.0 - (double)s.lr * t.decay[i]);
-  open8(fm, mc, __fmul_rn(mt, 1.0f / kTop));
-  open8(fv, vc, __fmul_rn(vt, 1.0f / kTop));
-  unsigned mbig = 0, vbig = 0;
+  // Whole blocks come through shared memory, kStages - 1 of them ahead of the
+  // one that is computed; the others are loaded where they are needed.
+  constexpr int kStages = 49152 / (int)sizeof(BlockStage<Tw, Tg>) > 4
+                              ? 4
+                              : 49152 / (int)sizeof(BlockStage<Tw, Tg>);
+  static_assert(kStages >= 2, "two blocks fit the shared memory");
+  __shared__ BlockStage<Tw, Tg> stages[kStages];
+  const int tid = threadIdx.x;
+  // starts the copies of the warp's block k, `ahead` of the pointers' one
+  auto copy = [&](int k, int ahead, int stage) {
+    const int o = ahead * kBlock;
+    if (k < whole) {
+      BlockStage<Tw, Tg>& b = stages[stage];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    moments(fm[j], fv[j], fg[j], c, s.scale);
-    fp[j] = stepped(fp[j], fm[j], fv[j], c, s, keep);
-    mbig = max(mbig, __float_as_uint(fm[j]) & 0x7fffffffu);
-    vbig = max(vbig, __float_as_uint(fv[j]) & 0x7fffffffu);
-  }
-  if (kMaster) store8(w + e, fp, left, w_whole);
-  store8(p + e, fp, left, p_whole);
-
-  mbig = __reduce_max_sync(0xffffffffu, mbig);
-  vbig = __reduce_max_sync(0xffffffffu, vbig);
-  float mtop = __uint_as_float(mbig), vtop = __uint_as_float(vbig);
-  const bool mgood = mbig < 0x7f800000u, vgood = vbig < 0x7f800000u;
-  if (mtop < kTinyTop) mtop = 0.0f;
-  if (vtop < kTinyTop) vtop = 0.0f;
-  const float minv = mgood && mtop > 0.0f ? __fmul_rn(__fdiv_rn(1.0f, mtop), kTop) : 0.0f;
-  const float vinv = vgood && vtop > 0.0f ? __fmul_rn(__fdiv_rn(1.0f, vtop), kTop) : 0.0f;
-
-  // 32 random bits a value: a full mix for the lane's eight, half a mix each
-  const uint32_t count = (uint32_t)(t.block[i] + block) * 32u + lane;
-  const uint32_t h = mix32(mix32(count) + s.key);
-  uint2 mo = make_uint2(0, 0), vo = make_uint2(0, 0);
+      for (int k = 0; k < (int)sizeof(Tw) / 2; ++k)
+        copy16(&b.w[k][tid], reinterpret_cast<const uint4*>(w + o) + k);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint32_t x = h + (uint32_t)j * kGolden;
-    x ^= x >> 17;
-    x *= 0xBB67AE85u;
-    x ^= x >> 15;
-    unsigned cm = close1(__fmul_rn(fabsf(fm[j]), minv), ((x & 0xffffu) << 4) + 8u);
-    unsigned cv = close1(__fmul_rn(fabsf(fv[j]), vinv), ((x >> 12) & 0xffff0u) + 8u);
-    if (fv[j] > 0.0f) cv = max(cv, 1u);  // a second moment above zero stays above it
-    if (fm[j] < 0.0f) cm |= 0x80u;
-    (j < 4 ? mo.x : mo.y) |= cm << (8 * (j & 3));
-    (j < 4 ? vo.x : vo.y) |= cv << (8 * (j & 3));
+      for (int k = 0; k < (int)sizeof(Tg) / 2; ++k)
+        copy16(&b.g[k][tid], reinterpret_cast<const uint4*>(g + o) + k);
+      copy8(&b.m[tid], m + o);
+      copy8(&b.v[tid], v + o);
+    }
+    copies_done();
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) copy(k, k, k);
+  // the lane's elements of a block that is not whole
+  auto some_of = [&](int k) {
+    const int64_t left = rest - k * kBlock - lane * 8;
+    return (int)(left < 0 ? 0 : left > 8 ? 8 : left);
+  };
+  // lane k holds the tops of the warp's block k, the old ones and then the new:
+  // one coalesced access for all of them (a load and a store of 4 bytes in the
+  // loop cost 20% of the whole step)
+  float mtops = 0.0f, vtops = 0.0f;
+  const bool has_tops = lane < here;
+  if (has_tops) {
+    mtops = item.mtop[block + lane];
+    vtops = item.vtop[block + lane];
   }
-  if (!mgood) mo = make_uint2(0, 0);
-  if (!vgood) vo = make_uint2(0, 0);
-  store8_codes(m + e, mo, left, m_whole);
-  store8_codes(v + e, vo, left, v_whole);
-  if (lane == 0) {
-    t.mtop[i][block] = mtop;
-    t.vtop[i][block] = vtop;
+  const StepValues s = step_values(values);
+  if (s.skip) {
+    wait_copies<0>();
+    return;
   }
+  const float keep = (float)(1.0 - (double)s.lr * item.decay);
+  const F2 scale = f2(s.scale, s.scale), beta1 = f2(c.beta1, c.beta1), rest1 = f2(c.rest1, c.rest1),
+           beta2 = f2(c.beta2, c.beta2), rest2 = f2(c.rest2, c.rest2), eps = f2(c.eps, c.eps),
+           root = f2(s.root, s.root), rate = f2(-s.rate, -s.rate), keep2 = f2(keep, keep),
+           zero = f2(c.zero, c.zero), lift = f2(0.015625f, 0.015625f);
+  int stage = 0;
+#pragma unroll 1
+  for (int k = 0; k < here; ++k) {
+    struct {
+      Raw8<Tw> p;
+      Raw8<Tg> g;
+      uint2 m, v;
+    } x;
+    wait_copies<kStages - 2>();
+    if (k < whole) {
+      const BlockStage<Tw, Tg>& b = stages[stage];
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(Tw) / 2; ++q) x.p.word[q] = b.w[q][tid];
+#pragma unroll
+      for (int q = 0; q < (int)sizeof(Tg) / 2; ++q) x.g.word[q] = b.g[q][tid];
+      x.m = b.m[tid];
+      x.v = b.v[tid];
+    } else {
+      const int some = some_of(k);
+      load8_some(x.p, (const Tw*)w, some);
+      load8_some(x.g, g, some);
+      x.m = load8_codes_some(m, some);
+      x.v = load8_codes_some(v, some);
+    }
+    // into the stage that the block before this one was read from
+    const int freed = stage == 0 ? kStages - 1 : stage - 1;
+    copy(k + kStages - 1, kStages - 1, freed);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    const float munit = __fmul_rn(__shfl_sync(0xffffffffu, mtops, k), 1.0f / kTop);
+    const float vunit = __fmul_rn(__shfl_sync(0xffffffffu, vtops, k), 1.0f / kTop);
+    const F2 munit2 = f2(munit, munit), vunit2 = f2(vunit, vunit);
+    F2 fm[4], fv[4];
+    float fp[8];
+    float mbig = 0.0f, vbig = 0.0f;
+    open4(fm[0], fm[1], x.m.x);
+    open4(fm[2], fm[3], x.m.y);
+    open4(fv[0], fv[1], x.v.x);
+    open4(fv[2], fv[3], x.v.y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      fm[j] = mul2(fm[j], munit2);
+      fv[j] = mul2(fv[j], vunit2);
+      const F2 fg = mul2(pair_of(x.g, j), scale);
+      // the assembler joins a packed product with the sum that takes it into one
+      // rounding; a product written as a sum with -0 is left alone
+      fm[j] = add2(fma2(fm[j], beta1, zero), fma2(fg, rest1, zero));
+      fv[j] = add2(fma2(fv[j], beta2, zero), fma2(mul2(fg, fg), rest2, zero));
+      const float2 a = halves(fm[j]), b = halves(fv[j]);
+      mbig = largest(mbig, a.x, a.y);
+      vbig = largest(vbig, b.x, b.y);
+      const float2 d = halves(fma2(f2(root_approx(b.x), root_approx(b.y)), root, eps));
+      const F2 move = mul2(fm[j], f2(inverse_approx(d.x), inverse_approx(d.y)));
+      const float2 q = halves(fma2(move, rate, mul2(pair_of(x.p, j), keep2)));
+      fp[2 * j] = q.x;
+      fp[2 * j + 1] = q.y;
+    }
+
+    const unsigned mmax = __reduce_max_sync(0xffffffffu, __float_as_uint(mbig) & 0x7fffffffu);
+    const unsigned vmax = __reduce_max_sync(0xffffffffu, __float_as_uint(vbig) & 0x7fffffffu);
+    // a top that is not finite or too small makes the block's codes zero; even
+    // lanes invert the one top, odd lanes the other
+    float mtop = __uint_as_float(mmax), vtop = __uint_as_float(vmax);
+    if (mtop < kTinyTop) mtop = 0.0f;
+    if (vtop < kTinyTop) vtop = 0.0f;
+    const float own = (lane & 1) ? vtop : mtop;
+    const float inverse = own > 0.0f && own < INFINITY ? __fmul_rn(__frcp_rn(own), kTop) : 0.0f;
+    const float minv = __shfl_sync(0xffffffffu, inverse, 0);
+    const float vinv = __shfl_sync(0xffffffffu, inverse, 1);
+    const F2 vinv2 = f2(vinv, vinv);
+
+    // 32 random bits a value: a full mix for the lane's eight, half a mix each
+    const uint32_t h = mix32(mix32(count) + s.key);
+    unsigned mw[8], vw[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t rm[2], rv[2];  // 16 bits each, at the bottom and at the top
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t y = h + (uint32_t)(2 * j + q) * kGolden;
+        y ^= y >> 17;
+        y *= 0xBB67AE85u;
+        const uint32_t z = y >> 15;
+        rm[q] = (y ^ z) & 0xffffu;
+        rv[q] = (y ^ z) & 0xffff0000u;
+      }
+      const float2 a = halves(fm[j]), b = halves(fv[j]);
+      const float2 ma = make_float2(__fmul_rn(fabsf(a.x), minv), __fmul_rn(fabsf(a.y), minv));
+      const float2 ml = halves(add2(f2(ma.x, ma.y), lift));
+      const F2 tb = fma2(fv[j], vinv2, zero);
+      const float2 va = halves(tb), vl = halves(add2(tb, lift));
+      const int m0 = rounding_word(ma.x, ml.x) + (int)(rm[0] << 4);
+      const int m1 = rounding_word(ma.y, ml.y) + (int)(rm[1] << 4);
+      int v0 = rounding_word(va.x, vl.x) + (int)(rv[0] >> 12);
+      int v1 = rounding_word(va.y, vl.y) + (int)(rv[1] >> 12);
+      // a second moment above zero stays above it
+      if (b.x > 0.0f) v0 = max(v0, kCodeOffset + (1 << 20));
+      if (b.y > 0.0f) v1 = max(v1, kCodeOffset + (1 << 20));
+      mw[2 * j] = upper_code(m0, c.sixteen) | (__float_as_uint(a.x) & 0x80000000u);
+      mw[2 * j + 1] = upper_code(m1, c.sixteen) | (__float_as_uint(a.y) & 0x80000000u);
+      vw[2 * j] = upper_code(v0, c.sixteen);
+      vw[2 * j + 1] = upper_code(v1, c.sixteen);
+    }
+    auto upper4 = [](const unsigned* u) {
+      return __byte_perm(__byte_perm(u[0], u[1], 0x0073), __byte_perm(u[2], u[3], 0x0073), 0x5410);
+    };
+    uint2 mo = make_uint2(upper4(mw), upper4(mw + 4)), vo = make_uint2(upper4(vw), upper4(vw + 4));
+    if (mmax >= 0x7f800000u) mo = make_uint2(0, 0);
+    if (vmax >= 0x7f800000u) vo = make_uint2(0, 0);
+    if (k < whole) {
+      if (kMaster) store_vec<8, kStream>((float*)w, fp);
+      store_vec<8, kStream>(p, fp);
+      __stcs(reinterpret_cast<uint2*>(m), mo);
+      __stcs(reinterpret_cast<uint2*>(v), vo);
+    } else {
+      const int some = some_of(k);
+      if (kMaster) store8_some((float*)w, fp, some);
+      store8_some(p, fp, some);
+      store8_codes_some(m, mo, some);
+      store8_codes_some(v, vo, some);
+    }
+    if (lane == k) {
+      mtops = mtop;
+      vtops = vtop;
+    }
+    p += kBlock;
+    w += kBlock;
+    g += kBlock;
+    m += kBlock;
+    v += kBlock;
+    count += 32;
+  }
+  if (has_tops) {
+    item.mtop[block + lane] = mtops;
+    item.vtop[block + lane] = vtops;
+  }
+  wait_copies<0>();
 }
 
-static_assert(sizeof(AdamTable) + kOtherParams <= kParamBytes, "the list fits the parameters");
-static_assert(sizeof(Adam8Table) + kOtherParams <= kParamBytes, "the list fits the parameters");
+static_assert(sizeof(AdamTable<kAdamCap>) + kOtherParams <= kParamBytes, "the list fits the parameters");
+static_assert(sizeof(Adam8Table<kAdam8Cap>) + kOtherParams <= kParamBytes, "the list fits the parameters");
 
 // ---------------------------------------------------------------------------
 // launchers
@@ -580,71 +814,102 @@ struct AdamLists {
   const double* weight_decay;
 };
 
-template <class Tp, class Tg, bool kMaster>
-inline int launch_adamw_lists(const AdamLists& l, const StepConst& c, const StepValues* values,
+template <class Tp, class Tg, bool kMaster, int kCap>
+inline int launch_adamw_parts(const AdamLists& l, const StepConst& c, const StepValues* values,
                               cudaStream_t stream) {
-  AdamTable t;
+  AdamTable<kCap> t;
   int64_t i = 0;
   while (i < l.count) {
     t.count = 0;
     int64_t tiles = 0;
-    for (; i < l.count && t.count < kAdamCap; ++i) {
+    for (; i < l.count && t.count < kCap; ++i) {
       if (l.sizes[i] == 0) continue;
       const int64_t more = ceil_div(l.sizes[i], (int64_t)kAdamTile);
       if (tiles + more > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
       const int k = t.count++;
-      t.p[k] = l.params[i];
-      t.g[k] = l.grads[i];
-      t.m[k] = static_cast<float*>(l.exp_avg[i]);
-      t.v[k] = static_cast<float*>(l.exp_avg_sq[i]);
-      t.w[k] = kMaster ? l.master[i] : nullptr;
-      t.n[k] = l.sizes[i];
-      t.decay[k] = l.weight_decay[i];
+      t.item[k] = {l.params[i],
+                   l.grads[i],
+                   static_cast<float*>(l.exp_avg[i]),
+                   static_cast<float*>(l.exp_avg_sq[i]),
+                   kMaster ? l.master[i] : nullptr,
+                   l.sizes[i],
+                   l.weight_decay[i]};
       t.first[k] = (uint32_t)tiles;
       tiles += more;
     }
     if (t.count == 0) break;
-    const int st = launch_dependent(adamw_kernel<Tp, Tg, kMaster>, dim3((unsigned)tiles),
+    const int st = launch_dependent(adamw_kernel<Tp, Tg, kMaster, kCap>, dim3((unsigned)tiles),
                                     dim3(kThreads), stream, t, values, c);
     if (st != LOOM_STATUS_OK) return st;
   }
   return LOOM_STATUS_OK;
 }
 
-template <class Tp, class Tg, bool kMaster>
-inline int launch_adamw8_lists(const AdamLists& l, const StepConst& c, const StepValues* values,
+template <class Tp, class Tg, bool kMaster, int kCap>
+inline int launch_adamw8_parts(const AdamLists& l, const StepConst& c, const StepValues* values,
                                cudaStream_t stream) {
-  Adam8Table t;
-  int64_t i = 0, block = 0;
+  Adam8Table<kCap> t;
+  int64_t i = 0, block = 0, all = 0;
+  for (int64_t k = 0; k < l.count; ++k) all += ceil_div(l.sizes[k], (int64_t)kBlock);
+  // one block per warp while these are fewer than the warps that the GPU holds
+  // at once, then as many as keep them all busy, up to kMaxWarpBlocks
+  int64_t per = all / (kSms * 4 * (kThreads / 32));
+  per = per < 1 ? 1 : per > kMaxWarpBlocks ? kMaxWarpBlocks : per;
+  t.warp_blocks = (int)per;
   while (i < l.count) {
     t.count = 0;
     int64_t tiles = 0;
-    for (; i < l.count && t.count < kAdam8Cap; ++i) {
+    for (; i < l.count && t.count < kCap; ++i) {
       if (l.sizes[i] == 0) continue;
       const int64_t blocks = ceil_div(l.sizes[i], (int64_t)kBlock);
-      const int64_t more = ceil_div(blocks, (int64_t)kTileBlocks);
+      const int64_t more = ceil_div(blocks, per * (kThreads / 32));
       if (tiles + more > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
       const int k = t.count++;
-      t.p[k] = l.params[i];
-      t.g[k] = l.grads[i];
-      t.m[k] = static_cast<uint8_t*>(l.exp_avg[i]);
-      t.v[k] = static_cast<uint8_t*>(l.exp_avg_sq[i]);
-      t.mtop[k] = l.exp_avg_top[i];
-      t.vtop[k] = l.exp_avg_sq_top[i];
-      t.w[k] = kMaster ? l.master[i] : nullptr;
-      t.n[k] = l.sizes[i];
-      t.decay[k] = l.weight_decay[i];
+      t.item[k] = {l.params[i],
+                   l.grads[i],
+                   static_cast<uint8_t*>(l.exp_avg[i]),
+                   static_cast<uint8_t*>(l.exp_avg_sq[i]),
+                   l.exp_avg_top[i],
+                   l.exp_avg_sq_top[i],
+                   kMaster ? l.master[i] : nullptr,
+                   l.sizes[i],
+                   l.weight_decay[i],
+                   (uint64_t)block};
       t.first[k] = (uint32_t)tiles;
-      t.block[k] = (uint32_t)block;
       tiles += more;
       block += blocks;
     }
     if (t.count == 0) break;
-    const int st = launch_dependent(adamw8_kernel<Tp, Tg, kMaster>, dim3((unsigned)tiles),
+    const int st = launch_dependent(adamw8_kernel<Tp, Tg, kMaster, kCap>, dim3((unsigned)tiles),
                                     dim3(kThreads), stream, t, values, c);
     if (st != LOOM_STATUS_OK) return st;
   }
   return LOOM_STATUS_OK;
+}
+
+template <class T>
+inline int launch_list_norm(int64_t count, const void* const* grads, const int64_t* sizes,
+                            float max_norm, float* out, void* workspace, cudaStream_t stream) {
+  return count <= kShortCap ? launch_list_norm_parts<T, kShortCap>(count, grads, sizes, max_norm,
+                                                                   out, workspace, stream)
+                            : launch_list_norm_parts<T, kNormCap>(count, grads, sizes, max_norm,
+                                                                  out, workspace, stream);
+}
+
+template <class Tp, class Tg, bool kMaster>
+inline int launch_adamw_lists(const AdamLists& l, const StepConst& c, const StepValues* values,
+                              cudaStream_t stream) {
+  return l.count <= kShortCap
+             ? launch_adamw_parts<Tp, Tg, kMaster, kShortCap>(l, c, values, stream)
+             : launch_adamw_parts<Tp, Tg, kMaster, kAdamCap>(l, c, values, stream);
+}
+
+template <class Tp, class Tg, bool kMaster>
+inline int launch_adamw8_lists(const AdamLists& l, const StepConst& c, const StepValues* values,
+                               cudaStream_t stream) {
+  return l.count <= kShortCap
+             ? launch_adamw8_parts<Tp, Tg, kMaster, kShortCap>(l, c, values, stream)
+             : launch_adamw8_parts<Tp, Tg, kMaster, kAdam8Cap>(l, c, values, stream);
 }
 
 }  // namespace loomb
