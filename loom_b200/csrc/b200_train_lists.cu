@@ -112,7 +112,7 @@ int adamw_impl(const AdamLists& l, int param_dtype, int grad_dtype, const float*
   c.sixteen = 16u;
   StepValues* values = reinterpret_cast<StepValues*>(loomb::workspace_base(workspace));
   const int st = loomb::launch_dependent(loomb::adamw_begin_kernel, dim3(1), dim3(32), stream,
-                                         values, lr, grad_scale, step, beta1, beta2, seed);
+                                         (size_t)0, values, lr, grad_scale, step, beta1, beta2, seed);
   if (st != LOOM_STATUS_OK) return st;
   switch (param_dtype) {
     case loomb::kF32: return launch_by_grad<kEight, float>(l, grad_dtype, c, values, stream);

@@ -5,6 +5,16 @@
 
 #include "loom_b200_block_norm.cuh"
 
+namespace loomb {
+#define LOOM_ROWS_ELSEWHERE(TX, TB)                                                             \
+  extern template int launch_block_norm<TX, TB>(const BlockNorm&, const BlockNormOut&,          \
+                                                cudaStream_t);                                  \
+  extern template int launch_block_norm_grad<TX, TB>(const BlockNorm&, BlockNormGrad, int64_t,  \
+                                                     void*, void*, void*, cudaStream_t);
+LOOM_ROW_TYPES(LOOM_ROWS_ELSEWHERE)
+#undef LOOM_ROWS_ELSEWHERE
+}  // namespace loomb
+
 namespace {
 
 using loomb::BlockNorm;
@@ -12,6 +22,8 @@ using loomb::BlockNormGrad;
 using loomb::BlockNormOut;
 
 bool aligned_to(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+
+bool stride_ok(int64_t s) { return s >= 0 && s < ((int64_t)1 << 31); }
 
 bool types_ok(int x_dtype, int h_dtype) {
   return loomb::valid_dtype(x_dtype) && loomb::valid_dtype(h_dtype) &&
@@ -47,8 +59,8 @@ bool common_ok(const BlockNorm& a, int64_t gate_rows, int64_t width, int x_dtype
     return false;
   const int bx = loomb::dtype_bytes(x_dtype), bh = loomb::dtype_bytes(h_dtype);
   return aligned_to(a.x, bx) && aligned_to(a.h, bh) && aligned_to(a.gate, bh) &&
-         aligned_to(a.post_weight, bh) && aligned_to(a.pre_weight, bh) && a.x_stride >= 0 &&
-         a.h_stride >= 0 && a.gate_stride >= 0;
+         aligned_to(a.post_weight, bh) && aligned_to(a.pre_weight, bh) && stride_ok(a.x_stride) &&
+         stride_ok(a.h_stride) && stride_ok(a.gate_stride);
 }
 
 int forward(BlockNorm a, int64_t gate_rows, int64_t width, int x_dtype, int h_dtype,
@@ -76,7 +88,7 @@ int backward(const BlockNorm& a, int64_t gate_rows, int64_t width, int x_dtype, 
   if (!aligned_to(b.dy, bx) || !aligned_to(b.dz, bh) || !aligned_to(b.dx, bx) ||
       !aligned_to(b.dh, bh) || !aligned_to(b.dgate, bh) || !aligned_to(dpost_weight, bh) ||
       !aligned_to(dpre_weight, bh) || !aligned_to(b.post_rstd, 4) || !aligned_to(b.pre_rstd, 4) ||
-      b.dy_stride < 0 || b.dz_stride < 0)
+      !stride_ok(b.dy_stride) || !stride_ok(b.dz_stride))
     return LOOM_STATUS_INVALID_ARGUMENT;
   if ((dpost_weight != nullptr && a.post_weight == nullptr) ||
       (dpre_weight != nullptr && a.pre_weight == nullptr))

@@ -13,7 +13,16 @@
 // HBM-bound: about a dozen operations an element on the 8 to 14 bytes that it
 // has to read and write.  So a row is read once and stays in registers between
 // its two sums: a row of up to 1024 elements belongs to one warp, a longer one
-// to one CTA.
+// to one CTA (a row group).  Row groups are persistent and walk the rows with a
+// stride; their next rows are on the way to shared memory (cp.async) while one
+// is computed, since a row's two sums are two barriers with nothing in flight.
+//
+// Groups of eight elements move as one access whatever the width: they lie at
+// multiples of eight elements from the array's start, not from the row's, so
+// a row begins `phase` = row * width mod 8 elements into its first group.  The
+// stride over the rows is a multiple of eight where the width is not, so each
+// row group has one phase for all its rows and holds the weights, and the
+// columns' sums of their gradients, at that phase in registers.
 #pragma once
 
 #include "loom_b200_launch.cuh"
@@ -67,120 +76,413 @@ __device__ __forceinline__ float row_sum(float v, float (*buf)[32], int& round) 
   return v;
 }
 
-// The NV groups of V elements of a row that a thread holds: group j starts at
-// (j * threads + thread) * V.
-template <int V, int NV, Cache kC, class T>
-__device__ __forceinline__ void load_row(float (&f)[NV][V], const T* p, int width) {
+// Three sums at once, the same bits in each of the row's threads: the halving
+// steps send two of four values away and keep two, then one and one, so that
+// three values take six exchanges a level.
+struct Sums3 {
+  float a, b, c;
+};
+__device__ __forceinline__ float fold8(float v) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int d = (j * blockDim.x + threadIdx.x) * V;
-    if (d < width) {
-      load_vec<V, kC>(f[j], p + d);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[j][i] = 0.0f;
-    }
-  }
+  for (int off = 4; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
 }
-template <int V, int NV, class T>
-__device__ __forceinline__ void store_row(T* p, const float (&f)[NV][V], int width) {
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int d = (j * blockDim.x + threadIdx.x) * V;
-    if (d < width) store_vec<V, kKeep>(p + d, f[j]);
+template <bool kWarp>
+__device__ __forceinline__ Sums3 row_sums(Sums3 s, float (*buf)[3][32], int& round) {
+  const int lane = threadIdx.x & 31;
+  const bool high = lane & 16, odd = lane & 8;
+  // lanes 0..15 keep a and b, lanes 16..31 keep c (and nothing)
+  const float first = (high ? s.c : s.a) + __shfl_xor_sync(0xffffffffu, high ? s.a : s.c, 16);
+  const float second = (high ? 0.0f : s.b) + __shfl_xor_sync(0xffffffffu, high ? s.b : 0.0f, 16);
+  // of these, lanes 0..7 keep a, 8..15 b, 16..23 c
+  float v = (odd ? second : first) + __shfl_xor_sync(0xffffffffu, odd ? first : second, 8);
+  v = fold8(v);
+  if constexpr (!kWarp) {
+    const int warps = blockDim.x >> 5;
+    float(*b)[32] = buf[round];
+    round ^= 1;
+    const int which = lane >> 3, at = lane & 7;
+    if (at == 0 && which < 3) b[which][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.0f;
+    if (which < 3)
+      for (int k = at; k < warps; k += 8) v += b[which][k];
+    v = fold8(v);
   }
-}
-template <int V, int NV, class T>
-__device__ __forceinline__ void load_weight(float (&f)[NV][V], const T* p, float offset,
-                                            int width) {
-  if (p == nullptr) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[j][i] = 1.0f;
-    return;
-  }
-  load_row<V, NV, kKeep>(f, p, width);
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[j][i] += offset;
+  return {__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 8),
+          __shfl_sync(0xffffffffu, v, 16)};
 }
 
-template <class Tx, class Tb, int V, int NV, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : 1024)
-block_norm_kernel(const BlockNorm a, const BlockNormOut o) {
+// ---------------------------------------------------------------------------
+// groups of eight elements, as four pairs
+
+struct Group {
+  F2 p[4];
+};
+
+__device__ __forceinline__ Group same(float v) {
+  Group g;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g.p[i] = f2(v, v);
+  return g;
+}
+__device__ __forceinline__ Group operator*(const Group& a, const Group& b) {
+  Group r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = mul2(a.p[i], b.p[i]);
+  return r;
+}
+__device__ __forceinline__ Group operator*(const Group& a, float b) {
+  Group r;
+  const F2 b2 = f2(b, b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = mul2(a.p[i], b2);
+  return r;
+}
+__device__ __forceinline__ Group operator+(const Group& a, const Group& b) {
+  Group r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = add2(a.p[i], b.p[i]);
+  return r;
+}
+// a * b + c
+__device__ __forceinline__ Group fma8(const Group& a, const Group& b, const Group& c) {
+  Group r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = fma2(a.p[i], b.p[i], c.p[i]);
+  return r;
+}
+__device__ __forceinline__ Group fma8(const Group& a, float b, const Group& c) {
+  Group r;
+  const F2 b2 = f2(b, b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = fma2(a.p[i], b2, c.p[i]);
+  return r;
+}
+__device__ __forceinline__ F2 dot8(const Group& a, const Group& b, F2 sum) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum = fma2(a.p[i], b.p[i], sum);
+  return sum;
+}
+
+// kEdge false: each thread's groups lie wholly in the row.  True: the first and
+// the last group may be partly outside, and threads may be left over.
+template <bool kEdge>
+__device__ __forceinline__ bool inside(int e, int width) {
+  return !kEdge || (e >= 0 && e + 8 <= width);
+}
+template <class T>
+__device__ __forceinline__ Group unpack(const Raw8<T>& r) {
+  Group g;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g.p[i] = pair_of(r, i);
+  return g;
+}
+// Zero outside the row (where a copy leaves a neighbour's values).
+template <bool kEdge>
+__device__ __forceinline__ Group within(Group g, int e, int width) {
+  if (!inside<kEdge>(e, width)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 f = halves(g.p[i]);
+      if (e + 2 * i < 0 || e + 2 * i >= width) f.x = 0.0f;
+      if (e + 2 * i + 1 < 0 || e + 2 * i + 1 >= width) f.y = 0.0f;
+      g.p[i] = f2(f.x, f.y);
+    }
+  }
+  return g;
+}
+// The group of a row that begins `e` elements after the row's start (which may
+// be before it), from any place; zero outside the row.
+template <class T>
+__device__ __forceinline__ Group load_group(const T* row, int e, int width) {
+  float f[8];
+  if (e >= 0 && e + 8 <= width && ((uintptr_t)(row + e) & 15u) == 0) {
+    load_vec<8, kKeep>(f, row + e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = e + i >= 0 && e + i < width ? widen(row[e + i]) : 0.0f;
+  }
+  Group g;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g.p[i] = f2(f[2 * i], f[2 * i + 1]);
+  return g;
+}
+// kPlaced: every whole group is at a 16-byte boundary.
+template <bool kPlaced, bool kEdge, class T>
+__device__ __forceinline__ void store_group(T* row, const Group& g, int e, int width) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 h = halves(g.p[i]);
+    f[2 * i] = h.x;
+    f[2 * i + 1] = h.y;
+  }
+  if (inside<kEdge>(e, width) && (kPlaced || ((uintptr_t)(row + e) & 15u) == 0)) {
+    store_vec<8, kKeep>(row + e, f);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (e + i >= 0 && e + i < width) row[e + i] = narrow<T>(f[i]);
+}
+// A weight with its offset; ones where there is no weight.
+template <class T>
+__device__ __forceinline__ Group load_weight(const T* w, float offset, int e, int width) {
+  if (w == nullptr) return same(1.0f);
+  Group g = load_group(w, e, width);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g.p[i] = add2(g.p[i], f2(offset, offset));
+  return g;
+}
+
+// The same as it lies in memory: 16-bit types in half the registers.
+template <class T>
+__device__ __forceinline__ Raw8<T> load_raw(const T* w, int e, int width) {
+  float f[8];
+  const Group g = w != nullptr ? load_group(w, e, width) : same(1.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 h = halves(g.p[i]);
+    f[2 * i] = h.x;
+    f[2 * i + 1] = h.y;
+  }
+  Raw8<T> r;
+  store_vec<8, kKeep>(reinterpret_cast<T*>(r.word), f);
+  return r;
+}
+// 16-byte words of a group of eight.
+template <class T>
+struct GroupWords {
+  static constexpr int value = (int)sizeof(T) / 2;
+};
+
+// Starts the copy of a group; `slot` words lie `pitch` apart.  Bytes past the
+// row's end are not read.  Bytes before its start (less than one group) are
+// read: they belong to the row before it, as the caller's strides are at least
+// a width and the phase is that of the row's own place.
+template <bool kEdge, class T>
+__device__ __forceinline__ void copy_group(uint4* slot, int pitch, const T* row, int e,
+                                           int width) {
+  const char* from = reinterpret_cast<const char*>(row + e);
+  const int bytes = (width - e) * (int)sizeof(T);
+#pragma unroll
+  for (int k = 0; k < GroupWords<T>::value; ++k) {
+    const int some = bytes - 16 * k;
+    if (!kEdge || some >= 16) {
+      copy16(slot + k * pitch, from + 16 * k);
+    } else {
+      copy16_some(slot + k * pitch, some > 0 ? from + 16 * k : from, some > 0 ? some : 0);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ Raw8<T> read_raw(const uint4* slot, int pitch) {
+  Raw8<T> r;
+#pragma unroll
+  for (int k = 0; k < GroupWords<T>::value; ++k) r.word[k] = slot[k * pitch];
+  return r;
+}
+
+__device__ __forceinline__ void wait_stage(int stages) {
+  if (stages == 4) {
+    wait_copies<2>();
+  } else if (stages == 3) {
+    wait_copies<1>();
+  } else {
+    wait_copies<0>();
+  }
+}
+
+__device__ __forceinline__ float total(F2 a) {
+  const float2 h = halves(a);
+  return h.x + h.y;
+}
+// Row starts: rows and strides are below 2^31, so one 32-bit product.
+template <class T>
+__device__ __forceinline__ const T* row_at(const void* p, int64_t row, int64_t stride) {
+  return static_cast<const T*>(p) + (uint64_t)(uint32_t)row * (uint32_t)stride;
+}
+template <class T>
+__device__ __forceinline__ T* row_at(void* p, int64_t row, int width) {
+  return static_cast<T*>(p) + (uint64_t)(uint32_t)row * (uint32_t)width;
+}
+
+// How the rows of one launch lie on threads.
+struct RowPlan {
+  int per;             // groups of eight per thread
+  bool warp;           // a warp per row, else a CTA
+  bool edge;           // groups partly outside of a row, or threads left over
+  int most;            // threads per CTA that the kernel is compiled for
+  unsigned threads;    // per row
+  int phased;          // groups lie at multiples of eight from the arrays' starts
+  int stages;          // rows on their way at once, 2 to 4; 0: loaded where they are needed
+  int64_t groups;      // row groups
+  int64_t rows;        // forward: rows of a row group, eight apart; 0: every groups-th row
+  size_t shared;       // bytes of the stages
+  dim3 block() const { return dim3(threads, warp ? kRowWarps : 1); }
+  dim3 grid() const { return dim3((unsigned)(warp ? (groups + kRowWarps - 1) / kRowWarps : groups)); }
+};
+
+// ---------------------------------------------------------------------------
+// forward
+
+// Stage of one thread: NV groups each of x, h and the gate (where it has a row
+// per row).
+template <class Tx, class Tb>
+struct ForwardStage {
+  static constexpr int x = 0, h = GroupWords<Tx>::value, gate = h + GroupWords<Tb>::value;
+  static constexpr int words = gate + GroupWords<Tb>::value;
+};
+
+template <class Tx, class Tb, bool kStaged, bool kEdge, int NV, bool kWarp, int kMost>
+__global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1)
+block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
+  using Stage = ForwardStage<Tx, Tb>;
+  extern __shared__ uint4 slots[];
   __shared__ float buf[2][32];
   int round = 0;
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= a.rows) return;
-  const int width = a.width;
+  const int64_t group = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (group >= plan.groups) return;  // whole warps of a CTA without barriers
+  const int width = a.width, threads = blockDim.x, stages = plan.stages;
   const float mean = 1.0f / (float)width;
-  float y[NV][V], u[NV][V], w[NV][V];
-  load_row<V, NV, kStream>(y, static_cast<const Tx*>(a.x) + row * a.x_stride, width);
-  if (a.h != nullptr) {
-    load_row<V, NV, kStream>(u, static_cast<const Tb*>(a.h) + row * a.h_stride, width);
-    float gate[NV][V];
-    load_weight<V, NV>(gate, a.gate == nullptr
-                                 ? nullptr
-                                 : static_cast<const Tb*>(a.gate) +
-                                       row / a.rows_per_gate * a.gate_stride,
-                       0.0f, width);
-    load_weight<V, NV>(w, static_cast<const Tb*>(a.post_weight), a.offset, width);
-    float rstd = 1.0f;
-    if (a.post_norm) {
-      float sum = 0.0f;
+  const int phase = kEdge && plan.phased ? (int)((group * width) & 7) : 0;
+  const int pitch = threads * blockDim.y;
+  const bool has_h = a.h != nullptr, row_gate = a.gate != nullptr && a.rows_per_gate == 1;
+  const bool run_gate = a.gate != nullptr && !row_gate;
+
+  int e[NV];
+  bool any[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    e[j] = (j * threads + (int)threadIdx.x) * 8 - phase;
+    any[j] = !kEdge || e[j] < width;
+  }
+  uint4* const mine = slots + threadIdx.y * threads + threadIdx.x;
+  auto slot = [&](int stage, int j, int part) {
+    return mine + ((stage * NV + j) * Stage::words + part) * pitch;
+  };
+  // All row groups walk the rows side by side (neighbouring rows at one time:
+  // 54 against 63 us for 8192 x 4096 bf16 rows), unless that would give each row
+  // another gate row; eight rows apart they still have one phase.
+  const int64_t step = plan.rows > 0 ? 8 : plan.groups;
+  const int64_t row0 = plan.rows > 0 ? (group >> 3) * 8 * plan.rows + (group & 7) : group;
+  const int64_t row1 = plan.rows > 0 ? min(a.rows, row0 + 8 * plan.rows) : a.rows;
+  auto copy = [&](int64_t row, int stage) {
+    if (row < row1) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!any[j]) continue;
+        copy_group<kEdge>(slot(stage, j, Stage::x), pitch, row_at<Tx>(a.x, row, a.x_stride), e[j],
+                          width);
+        if (has_h)
+          copy_group<kEdge>(slot(stage, j, Stage::h), pitch, row_at<Tb>(a.h, row, a.h_stride),
+                            e[j], width);
+        if (row_gate)
+          copy_group<kEdge>(slot(stage, j, Stage::gate), pitch,
+                            row_at<Tb>(a.gate, row, a.gate_stride), e[j], width);
+      }
+    }
+    copies_done();
+  };
+  if (kStaged)
+    for (int s = 0; s < stages - 1; ++s) copy(row0 + step * s, s);
+  Group w_post[NV], w_pre[NV], gate[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    w_post[j] = load_weight(static_cast<const Tb*>(a.post_weight), a.offset, e[j], width);
+    w_pre[j] = load_weight(static_cast<const Tb*>(a.pre_weight), a.offset, e[j], width);
+    gate[j] = same(1.0f);
+  }
+
+  int64_t run_end = 0;  // of the rows that the gate in registers serves
+  int stage = 0;
+  for (int64_t row = row0; row < row1; row += step) {
+    Group y[NV], u[NV];
+    if (run_gate && row >= run_end) {
+      const uint32_t run = (uint32_t)row / (uint32_t)a.rows_per_gate;
+      run_end = (run + 1) * a.rows_per_gate;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum = fmaf(u[j][i], u[j][i], sum);
-      sum = row_sum<kWarp>(sum, buf, round);
-      rstd = 1.0f / sqrtf(fmaf(sum, mean, a.eps));
-      if (threadIdx.x == 0 && o.post_rstd != nullptr) o.post_rstd[row] = rstd;
+        gate[j] = load_group(row_at<Tb>(a.gate, run, a.gate_stride), e[j], width);
     }
+    if (kStaged) wait_stage(stages);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!kStaged) {
+        y[j] = load_group(row_at<Tx>(a.x, row, a.x_stride), e[j], width);
+        if (has_h) u[j] = load_group(row_at<Tb>(a.h, row, a.h_stride), e[j], width);
+        if (row_gate) gate[j] = load_group(row_at<Tb>(a.gate, row, a.gate_stride), e[j], width);
+      } else if (any[j]) {
+        y[j] = within<kEdge>(unpack(read_raw<Tx>(slot(stage, j, Stage::x), pitch)), e[j], width);
+        if (has_h)
+          u[j] = within<kEdge>(unpack(read_raw<Tb>(slot(stage, j, Stage::h), pitch)), e[j], width);
+        if (row_gate)
+          gate[j] = within<kEdge>(unpack(read_raw<Tb>(slot(stage, j, Stage::gate), pitch)), e[j],
+                                  width);
+      } else {
+        y[j] = u[j] = same(0.0f);
+      }
+    }
+    if (kStaged) {
+      // into the stage that the row before this one was read from
+      copy(row + step * (stages - 1), stage == 0 ? stages - 1 : stage - 1);
+      stage = stage == stages - 1 ? 0 : stage + 1;
+    }
+    if (has_h) {
+      float rstd = 1.0f;
+      if (a.post_norm) {
+        F2 sum = f2(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) sum = dot8(u[j], u[j], sum);
+        rstd = rsqrtf(fmaf(row_sum<kWarp>(total(sum), buf, round), mean, a.eps));
+        if (threadIdx.x == 0 && o.post_rstd != nullptr) o.post_rstd[row] = rstd;
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        y[j] = fma8(u[j] * rstd * w_post[j] * gate[j], a.branch_scale, y[j] * a.residual_scale);
+        if (any[j])
+          store_group<kStaged, kEdge>(row_at<Tx>(o.y, row, width), y[j], e[j], width);
+      }
+    }
+    if (!a.pre_norm) continue;
+    F2 sum = f2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) sum = dot8(y[j], y[j], sum);
+    const float rstd = rsqrtf(fmaf(row_sum<kWarp>(total(sum), buf, round), mean, a.eps));
+    if (threadIdx.x == 0 && o.pre_rstd != nullptr) o.pre_rstd[row] = rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float b = gate[j][i] * (u[j][i] * rstd * w[j][i]);
-        y[j][i] = fmaf(a.branch_scale, b, a.residual_scale * y[j][i]);
-      }
-    store_row<V, NV>(static_cast<Tx*>(o.y) + row * width, y, width);
+      if (any[j])
+        store_group<kStaged, kEdge>(row_at<Tb>(o.z, row, width), y[j] * rstd * w_pre[j], e[j],
+                                    width);
   }
-  if (!a.pre_norm) return;
-  load_weight<V, NV>(w, static_cast<const Tb*>(a.pre_weight), a.offset, width);
-  float sum = 0.0f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum = fmaf(y[j][i], y[j][i], sum);
-  sum = row_sum<kWarp>(sum, buf, round);
-  const float rstd = 1.0f / sqrtf(fmaf(sum, mean, a.eps));
-  if (threadIdx.x == 0 && o.pre_rstd != nullptr) o.pre_rstd[row] = rstd;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) y[j][i] = y[j][i] * rstd * w[j][i];
-  store_row<V, NV>(static_cast<Tb*>(o.z) + row * width, y, width);
+  if (kStaged) wait_copies<0>();
 }
 
 // ---------------------------------------------------------------------------
 // gradients
 //
 //   n = y pre_rstd, t = dz w_pre:        d = dy + pre_rstd (t - n mean(t n)),  dx = residual_scale d
-//   k = h post_rstd, e = branch gate d:  dh = post_rstd (e w_post - k mean(e w_post k))
-//   dgate = branch d k w_post,  dpost_weight = sum over rows of e k,  dpre_weight = of dz n
+//   k = h post_rstd, q = branch gate d:  dh = post_rstd (q w_post - k mean(q w_post k))
+//   dgate = branch d k w_post,  dpost_weight = sum over rows of q k,  dpre_weight = of dz n
 //
-// The rows are cut into chunks that lie within one gate row's run of rows, and
-// a fixed number of row groups (CTAs or warps) walk the chunks.  A group keeps
-// its columns' sums of the weights' gradients in fp32 registers over all its
-// rows and leaves them as one row of the workspace; a gate row's gradient is
-// summed over its run, written where the run is one chunk and left as a
-// partial row else.  A second kernel adds the partial rows in a fixed order.
-
-constexpr int kGradCtas = 296;          // two per SM
+// The second mean would wait for the first.  With f = dy + pre_rstd t and
+// c = branch gate w_post, q w_post = c d = c (f - pre_rstd mean(t n) n), so that
+//
+//   mean(q w_post k) = mean(c f k) - pre_rstd mean(t n) mean(c n k)
+//
+// and a row takes one round of three sums; the terms are those that d itself
+// is made of, so nothing cancels that does not in d.
+//
+// A row group keeps its columns' sums of the weights' gradients in fp32
+// registers over all its rows and leaves them as one row of the workspace.
+// Where a gate row serves a run of rows, the run's rows are dealt to
+// `chunks_per_gate` chunks, and a row group walks whole chunks: the gate row's
+// gradient is written where the run is one chunk, and left as a partial row
+// else.  A second kernel adds the partial rows in a fixed order.
 
 struct BlockNormGrad {
   const float* post_rstd;
@@ -194,117 +496,231 @@ struct BlockNormGrad {
   float* pre_rows;               // partial rows: one per row group
   float* post_rows;
   float* gate_rows;              // one per chunk, where a gate row has several
-  int64_t chunks;
+  int64_t chunks;                // runs * chunks_per_gate; without runs, the row groups
+  int64_t run_rows;              // rows of a run
   int chunks_per_gate;
 };
 
-template <class Tx, class Tb, int V, int NV, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? 32 * kRowWarps : 1024)
-block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b) {
+// The rows of a row group, chunk after chunk.
+struct RowWalk {
+  int64_t chunk, row, end;
+  __device__ __forceinline__ void enter(const BlockNormGrad& b) {
+    if (chunk >= b.chunks) {
+      row = -1;
+      return;
+    }
+    const uint32_t run = (uint32_t)chunk / (uint32_t)b.chunks_per_gate;  // below 2^31, all
+    row = run * b.run_rows + (chunk - (int64_t)run * b.chunks_per_gate);
+    end = (run + 1) * b.run_rows;
+  }
+  __device__ __forceinline__ void next(const BlockNormGrad& b, int64_t groups) {
+    if (row < 0) return;
+    row += b.chunks_per_gate;
+    if (row >= end) {
+      chunk += groups;
+      enter(b);
+    }
+  }
+};
+
+template <class Tx, class Tb>
+struct GradStage {
+  static constexpr int y = 0, dy = GroupWords<Tx>::value, h = dy + GroupWords<Tx>::value;
+  static constexpr int dz = h + GroupWords<Tb>::value, gate = dz + GroupWords<Tb>::value;
+  static constexpr int words = gate + GroupWords<Tb>::value;
+};
+
+// Where the gate's rows are: none, one per row, one per run of rows.
+enum Gate : int { kNoGate = 0, kRowGate = 1, kRunGate = 2 };
+
+// kWhole: both norms, h and dy are there (tests of them in the loop are a third
+// of the instructions: 103 against 119 us for 8192 x 4096 bf16 rows).
+template <class Tx, class Tb, bool kStaged, bool kEdge, int NV, bool kWarp, int kMost, Gate kGate,
+          bool kWhole>
+__global__ void __launch_bounds__(kMost)
+block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan plan) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
-  __shared__ float buf[2][32];
+  using Stage = GradStage<Tx, Tb>;
+  extern __shared__ uint4 slots[];
+  __shared__ float buf[2][3][32];
   int round = 0;
-  const int width = a.width;
-  const float mean = 1.0f / (float)width;
   const int64_t group = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const int64_t groups = (int64_t)gridDim.x * blockDim.y;
-  float w_pre[NV][V], w_post[NV][V], s_pre[NV][V], s_post[NV][V];
-  load_weight<V, NV>(w_pre, static_cast<const Tb*>(a.pre_weight), a.offset, width);
-  load_weight<V, NV>(w_post, static_cast<const Tb*>(a.post_weight), a.offset, width);
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < V; ++i) s_pre[j][i] = s_post[j][i] = 0.0f;
+  const int64_t groups = plan.groups;
+  if (group >= groups) return;  // whole warps of a CTA without barriers
+  const int width = a.width, threads = blockDim.x, stages = plan.stages;
+  const float mean = 1.0f / (float)width;
+  const int phase = kEdge && plan.phased ? (int)((group * width) & 7) : 0;
+  const int pitch = threads * blockDim.y;
+  const bool has_h = kWhole || a.h != nullptr, has_dy = kWhole || b.dy != nullptr;
+  const bool pre_norm = kWhole || a.pre_norm, post_norm = kWhole || (a.post_norm && has_h);
 
-  for (int64_t chunk = group; chunk < b.chunks; chunk += groups) {
-    const int64_t run = chunk / b.chunks_per_gate;
-    const int64_t part = chunk - run * b.chunks_per_gate;
-    const int64_t row0 = run * a.rows_per_gate + a.rows_per_gate * part / b.chunks_per_gate;
-    const int64_t row1 = run * a.rows_per_gate + a.rows_per_gate * (part + 1) / b.chunks_per_gate;
-    float gate[NV][V], s_gate[NV][V];
-    load_weight<V, NV>(gate, a.gate == nullptr
-                                 ? nullptr
-                                 : static_cast<const Tb*>(a.gate) + run * a.gate_stride,
-                       0.0f, width);
+  int e[NV];
+  bool any[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    e[j] = (j * threads + (int)threadIdx.x) * 8 - phase;
+    any[j] = !kEdge || e[j] < width;
+  }
+  uint4* const mine = slots + threadIdx.y * threads + threadIdx.x;
+  auto slot = [&](int stage, int j, int part) {
+    return mine + ((stage * NV + j) * Stage::words + part) * pitch;
+  };
+  auto copy = [&](int64_t row, int stage) {
+    if (row >= 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s_gate[j][i] = 0.0f;
-    for (int64_t row = row0; row < row1; ++row) {
-      float y[NV][V], d[NV][V];
-      if (b.dy != nullptr) {
-        load_row<V, NV, kStream>(d, static_cast<const Tx*>(b.dy) + row * b.dy_stride, width);
-      } else {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) d[j][i] = 0.0f;
-      }
-      float h[NV][V];
-      if (a.h != nullptr)
-        load_row<V, NV, kStream>(h, static_cast<const Tb*>(a.h) + row * a.h_stride, width);
-      if (a.pre_norm) {
-        float t[NV][V];
-        load_row<V, NV, kStream>(y, static_cast<const Tx*>(a.x) + row * a.x_stride, width);
-        load_row<V, NV, kStream>(t, static_cast<const Tb*>(b.dz) + row * b.dz_stride, width);
-        const float rstd = b.pre_rstd[row];
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            y[j][i] *= rstd;
-            s_pre[j][i] = fmaf(t[j][i], y[j][i], s_pre[j][i]);
-            t[j][i] *= w_pre[j][i];
-            sum = fmaf(t[j][i], y[j][i], sum);
-          }
-        sum = row_sum<kWarp>(sum, buf, round) * mean;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            d[j][i] = fmaf(rstd, fmaf(-y[j][i], sum, t[j][i]), d[j][i]);
-      }
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[j][i] = a.residual_scale * d[j][i];
-      store_row<V, NV>(static_cast<Tx*>(b.dx) + row * width, y, width);
-      if (a.h == nullptr) continue;
-      const float rstd = a.post_norm ? b.post_rstd[row] : 1.0f;
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          h[j][i] *= rstd;
-          d[j][i] *= a.branch_scale;
-          s_gate[j][i] = fmaf(d[j][i], h[j][i] * w_post[j][i], s_gate[j][i]);
-          d[j][i] *= gate[j][i];
-          s_post[j][i] = fmaf(d[j][i], h[j][i], s_post[j][i]);
-          d[j][i] *= w_post[j][i];
-          sum = fmaf(d[j][i], h[j][i], sum);
+      for (int j = 0; j < NV; ++j) {
+        if (!any[j]) continue;
+        if (pre_norm) {
+          copy_group<kEdge>(slot(stage, j, Stage::y), pitch, row_at<Tx>(a.x, row, a.x_stride),
+                            e[j], width);
+          copy_group<kEdge>(slot(stage, j, Stage::dz), pitch, row_at<Tb>(b.dz, row, b.dz_stride),
+                            e[j], width);
         }
-      if (a.post_norm) {
-        sum = row_sum<kWarp>(sum, buf, round) * mean;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) d[j][i] = rstd * fmaf(-h[j][i], sum, d[j][i]);
+        if (has_dy)
+          copy_group<kEdge>(slot(stage, j, Stage::dy), pitch, row_at<Tx>(b.dy, row, b.dy_stride),
+                            e[j], width);
+        if (has_h)
+          copy_group<kEdge>(slot(stage, j, Stage::h), pitch, row_at<Tb>(a.h, row, a.h_stride),
+                            e[j], width);
+        if (kGate == kRowGate)
+          copy_group<kEdge>(slot(stage, j, Stage::gate), pitch,
+                            row_at<Tb>(a.gate, row, a.gate_stride), e[j], width);
       }
-      store_row<V, NV>(static_cast<Tb*>(b.dh) + row * width, d, width);
     }
-    if (b.dgate != nullptr) {
-      if (b.chunks_per_gate == 1) {
-        store_row<V, NV>(static_cast<Tb*>(b.dgate) + run * width, s_gate, width);
-      } else {
-        store_row<V, NV>(b.gate_rows + chunk * width, s_gate, width);
+    copies_done();
+  };
+  // a group of this row, from its stage or from memory
+  auto fetch = [&](auto type, const void* p, int64_t row, int64_t stride, int stage, int j,
+                   int part) {
+    using T = decltype(type);
+    if (!kStaged) return load_group(row_at<T>(p, row, stride), e[j], width);
+    if (!any[j]) return same(0.0f);
+    return within<kEdge>(unpack(read_raw<T>(slot(stage, j, part), pitch)), e[j], width);
+  };
+  RowWalk ahead = {group, 0, 0}, now = {group, 0, 0};
+  ahead.enter(b);
+  now.enter(b);
+  for (int s = 0; kStaged && s < stages - 1; ++s) {
+    copy(ahead.row, s);
+    ahead.next(b, groups);
+  }
+  Raw8<Tb> gate[NV];
+  Group w_post[NV], w_pre[NV], s_pre[NV], s_post[NV], s_gate[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    w_post[j] = load_weight(static_cast<const Tb*>(a.post_weight), a.offset, e[j], width);
+    w_pre[j] = load_weight(static_cast<const Tb*>(a.pre_weight), a.offset, e[j], width);
+    gate[j] = load_raw(static_cast<const Tb*>(nullptr), e[j], width);
+    s_pre[j] = s_post[j] = s_gate[j] = same(0.0f);
+  }
+
+  int64_t chunk = -1;
+  int stage = 0;
+  while (now.row >= 0) {
+    const int64_t row = now.row;
+    if (kGate == kRunGate && now.chunk != chunk) {
+      chunk = now.chunk;
+      const Tb* from = row_at<Tb>(
+          a.gate, (uint32_t)chunk / (uint32_t)b.chunks_per_gate, a.gate_stride);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        gate[j] = load_raw(from, e[j], width);
+        s_gate[j] = same(0.0f);
+      }
+    }
+    const float pre_rstd = pre_norm ? b.pre_rstd[row] : 1.0f;
+    const float post_rstd = post_norm ? b.post_rstd[row] : 1.0f;
+    if (kStaged) {
+      wait_stage(stages);
+      // into the stage that the row before this one was read from
+      copy(ahead.row, stage == 0 ? stages - 1 : stage - 1);
+      ahead.next(b, groups);
+    }
+    Group f[NV], n[NV], k[NV];
+    F2 tn = f2(0.0f, 0.0f), cfk = tn, cnk = tn;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      f[j] = n[j] = k[j] = same(0.0f);
+      if (has_dy) f[j] = fetch(Tx(), b.dy, row, b.dy_stride, stage, j, Stage::dy);
+      if (pre_norm) {
+        n[j] = fetch(Tx(), a.x, row, a.x_stride, stage, j, Stage::y) * pre_rstd;
+        Group t = fetch(Tb(), b.dz, row, b.dz_stride, stage, j, Stage::dz);
+        s_pre[j] = fma8(t, n[j], s_pre[j]);
+        t = t * w_pre[j];
+        tn = dot8(t, n[j], tn);
+        f[j] = fma8(t, pre_rstd, f[j]);
+      }
+      if (has_h) {
+        k[j] = fetch(Tb(), a.h, row, a.h_stride, stage, j, Stage::h) * post_rstd;
+        if (kGate == kRowGate) {
+          if (!kStaged) gate[j] = load_raw(row_at<Tb>(a.gate, row, a.gate_stride), e[j], width);
+          else if (any[j]) gate[j] = read_raw<Tb>(slot(stage, j, Stage::gate), pitch);
+        }
+        if (post_norm) {
+          Group c = w_post[j] * k[j];
+          if (kGate != kNoGate) c = c * within<kEdge>(unpack(gate[j]), e[j], width);
+          cfk = dot8(c, f[j], cfk);
+          cnk = dot8(c, n[j], cnk);
+        }
+      }
+    }
+    float pull = 0.0f, post_pull = 0.0f;  // the means, with their signs
+    if (pre_norm || post_norm) {
+      const Sums3 s = row_sums<kWarp>({total(tn), total(cfk), total(cnk)}, buf, round);
+      pull = -pre_rstd * (s.a * mean);
+      post_pull = -(fmaf(pull, s.c, s.b) * (mean * a.branch_scale));
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const Group d = fma8(n[j], pull, f[j]);
+      if (any[j])
+        store_group<kStaged, kEdge>(row_at<Tx>(b.dx, row, width), d * a.residual_scale, e[j],
+                                    width);
+      if (has_h) {
+        const Group scaled = d * a.branch_scale, own = scaled * k[j];
+        Group through = scaled, sum = own;  // with the gate
+        if (kGate != kNoGate) {
+          const Group g = within<kEdge>(unpack(gate[j]), e[j], width);
+          through = scaled * g;
+          sum = own * g;
+        }
+        if (kGate == kRowGate) {
+          if (any[j])
+            store_group<kStaged, kEdge>(row_at<Tb>(b.dgate, row, width), own * w_post[j], e[j], width);
+        } else if (kGate == kRunGate) {
+          s_gate[j] = fma8(own, w_post[j], s_gate[j]);
+        }
+        s_post[j] = s_post[j] + sum;
+        const Group dh = fma8(k[j], post_pull, through * w_post[j]) * post_rstd;
+        if (any[j])
+          store_group<kStaged, kEdge>(row_at<Tb>(b.dh, row, width), dh, e[j], width);
+      }
+    }
+    stage = stage == stages - 1 ? 0 : stage + 1;
+    now.next(b, groups);
+    if (kGate == kRunGate && now.chunk != chunk) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (!any[j]) continue;
+        if (b.chunks_per_gate == 1) {
+          store_group<false, true>(row_at<Tb>(b.dgate, chunk, width), s_gate[j], e[j], width);
+        } else {
+          store_group<false, true>(row_at<float>(b.gate_rows, chunk, width), s_gate[j], e[j],
+                                   width);
+        }
       }
     }
   }
-  if (b.pre_rows != nullptr) store_row<V, NV>(b.pre_rows + group * width, s_pre, width);
-  if (b.post_rows != nullptr) store_row<V, NV>(b.post_rows + group * width, s_post, width);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (!any[j]) continue;
+    if (b.pre_rows != nullptr)
+      store_group<false, true>(b.pre_rows + group * width, s_pre[j], e[j], width);
+    if (b.post_rows != nullptr)
+      store_group<false, true>(b.post_rows + group * width, s_post[j], e[j], width);
+  }
+  if (kStaged) wait_copies<0>();
 }
 
 // Sums of partial rows by column: job 0 the pre weight's, job 1 the post
@@ -334,6 +750,7 @@ __global__ void __launch_bounds__(256) block_norm_sums_kernel(const RowSums s, i
   float sum = 0.0f;
   if (d < s.width) {
     const float* p = s.rows[kind] + line * count * s.width + d;
+#pragma unroll 8
     for (int64_t r = stride; r < count; r += 8) sum += p[r * s.width];
   }
   part[stride][lane] = sum;
@@ -348,140 +765,251 @@ __global__ void __launch_bounds__(256) block_norm_sums_kernel(const RowSums s, i
 // ---------------------------------------------------------------------------
 // launchers
 
-// Whether 8 elements at a time can be moved of every row of this array.
-inline bool rows_by_8(const void* p, int64_t stride, int width) {
-  return p == nullptr || (((uintptr_t)p & 15u) == 0 && stride % 8 == 0 && width % 8 == 0);
+constexpr int kSmCount = 148;                  // of a B200
+constexpr size_t kStageBytes = 220 * 1024;     // shared memory of an SM that stages may take
+
+// Whether an array's rows have the phase of contiguous ones: copies then find
+// every group at a 16-byte boundary, and what lies before a row's first
+// element is the row before it.
+inline bool in_phase(const void* p, int64_t stride, int64_t rows, int width) {
+  return p == nullptr || (((uintptr_t)p & 15u) == 0 &&
+                          (rows <= 1 || (stride >= width && (stride - width) % 8 == 0)));
 }
 
-// How the rows of one launch lie on threads.
-struct RowShape {
-  int vec, per;        // elements per access, accesses per thread
-  bool warp;           // a warp per row
-  unsigned threads;    // per row
-  dim3 block() const { return dim3(threads, warp ? kRowWarps : 1); }
-};
-
-inline RowShape row_shape(int width, bool by8) {
-  RowShape s;
-  s.vec = by8 ? 8 : 1;
-  const int units = by8 ? width / 8 : width;
-  const int warp_most = by8 ? 4 : 8;
-  s.warp = units <= 32 * warp_most;
-  if (s.warp) {
-    s.per = by8 ? (units <= 32 ? 1 : units <= 64 ? 2 : 4) : 8;
-    s.threads = 32;
+// `words`: 16-byte words of a stage per thread and group of eight; `per`: groups
+// per thread of a staged CTA; `resident`: threads per SM that the kernel's
+// registers allow, about; `warp_units`: groups of eight that a warp takes at
+// most.  `stage`: whether rows come through stages at all.
+inline RowPlan row_plan(int width, bool phased, bool stage, int words, int resident, int per,
+                        int warp_units) {
+  RowPlan s = {};
+  s.phased = phased;
+  const int units = phased && width % 8 != 0 ? (width + 14) / 8 : (width + 7) / 8;
+  for (int staged = phased && stage ? 1 : 0;; --staged) {
+    s.warp = units <= warp_units;
+    if (s.warp) {
+      s.per = units <= 32 ? 1 : units <= 64 ? 2 : 4;
+      s.threads = 32;
+      s.most = 32 * kRowWarps;
+    } else {
+      if (staged) {
+        s.per = per;
+        s.most = units <= 512 ? 512 / per : units <= 1024 ? 1024 / per : 1024;
+      } else {
+        s.per = units <= 1024 ? 1 : 4;
+        s.most = units <= 512 ? 512 : 1024;
+      }
+      s.threads = (unsigned)(ceil_div(ceil_div(units, s.per), 32) * 32);
+    }
+    const int threads = (int)s.threads * (s.warp ? kRowWarps : 1);
+    int ctas = resident / threads;
+    if (ctas < 1) ctas = 1;
+    s.edge = !staged || width % 8 != 0 || units != (int)s.threads * s.per;
+    if (staged) {
+      const size_t bytes = (size_t)s.per * words * 16 * threads;
+      // wider than the staged kernels go, or than shared memory holds two rows of
+      if (threads > s.most || 2 * bytes > kStageBytes) continue;
+      if (2 * bytes * ctas > kStageBytes) ctas = (int)(kStageBytes / (2 * bytes));
+      const size_t fit = kStageBytes / ctas / bytes;
+      s.stages = fit < 4 ? (int)fit : 4;
+      s.shared = (size_t)s.stages * bytes;
+    } else if (units > 4096) {
+      // an odd width whose shifted groups pass the widest CTA: unshifted
+      return row_plan(width, false, false, words, resident, per, warp_units);
+    }
+    s.groups = (int64_t)kSmCount * ctas * (s.warp ? kRowWarps : 1);
     return s;
   }
-  s.per = by8 ? (units <= 1024 ? 1 : units <= 2048 ? 2 : 4) : (units <= 8192 ? 8 : 32);
-  s.threads = (unsigned)(ceil_div(ceil_div(units, s.per), 32) * 32);
-  return s;
 }
 
-// Calls f with the shape as constants.
-template <class F>
-inline int with_shape(const RowShape& s, const F& f) {
-  using std::integral_constant;
-  if (s.vec == 8) {
-    if (s.warp) {
-      if (s.per == 1) return f(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
-      if (s.per == 2) return f(integral_constant<int, 8>(), integral_constant<int, 2>(), std::true_type());
-      return f(integral_constant<int, 8>(), integral_constant<int, 4>(), std::true_type());
-    }
-    if (s.per == 1) return f(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
-    if (s.per == 2) return f(integral_constant<int, 8>(), integral_constant<int, 2>(), std::false_type());
-    return f(integral_constant<int, 8>(), integral_constant<int, 4>(), std::false_type());
+// A row group that takes several rows of one phase steps by a multiple of
+// eight rows, unless every row has it.
+inline int64_t step_groups(int64_t groups, int64_t rows, int width, bool phased) {
+  if (groups >= rows) return rows;
+  return phased && width % 8 != 0 && groups >= 8 ? groups / 8 * 8 : groups;
+}
+
+template <class Kern, class... Args>
+inline int launch_rows(Kern kernel, const RowPlan& s, cudaStream_t stream, const Args&... args) {
+  // without the attribute 48 KiB, the kernel's own 256 bytes among them
+  if (s.shared > 47 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.shared) !=
+          cudaSuccess) {
+    cudaGetLastError();
+    return LOOM_STATUS_CUDA_ERROR;
   }
-  if (s.warp) return f(integral_constant<int, 1>(), integral_constant<int, 8>(), std::true_type());
-  if (s.per == 8) return f(integral_constant<int, 1>(), integral_constant<int, 8>(), std::false_type());
-  return f(integral_constant<int, 1>(), integral_constant<int, 32>(), std::false_type());
+  return launch_dependent(kernel, s.grid(), s.block(), stream, s.shared, args..., s);
+}
+
+// Calls f with the plan as constants; kPer 2 is the forward pass's, 1 the
+// backward's, whose warps take at most two groups a lane.
+template <int kPer, class F>
+inline int with_plan(const RowPlan& s, const F& f) {
+  using std::integral_constant;
+  const std::true_type yes;
+  const std::false_type no;
+  const integral_constant<int, 1> one;
+  const integral_constant<int, 2> two;
+  const integral_constant<int, 4> four;
+  const integral_constant<int, 32 * kRowWarps> warps;
+  const integral_constant<int, 512> half;
+  const integral_constant<int, 1024> full;
+  auto by_warps = [&](auto staged, auto edge) {
+    if constexpr (kPer > 1)
+      if (s.per == 4) return f(staged, edge, four, yes, warps);
+    return s.per == 1 ? f(staged, edge, one, yes, warps) : f(staged, edge, two, yes, warps);
+  };
+  if (s.stages == 0) {
+    if (s.warp) return by_warps(no, yes);
+    if (s.per == 4) return f(no, yes, four, no, full);
+    return s.most == 512 ? f(no, yes, one, no, half) : f(no, yes, one, no, full);
+  }
+  auto staged = [&](auto edge) {
+    if (s.warp) return by_warps(yes, edge);
+    const integral_constant<int, kPer> per;
+    const integral_constant<int, 512 / kPer> narrow_cta;
+    const integral_constant<int, 1024 / kPer> wide_cta;
+    if (s.most == 512 / kPer) return f(yes, edge, per, no, narrow_cta);
+    if (s.most == 1024 / kPer) return f(yes, edge, per, no, wide_cta);
+    if constexpr (kPer > 1) return f(yes, edge, per, no, full);
+    return (int)LOOM_STATUS_CUDA_ERROR;
+  };
+  return s.edge ? staged(yes) : staged(no);
 }
 
 template <class Tx, class Tb>
-inline int launch_block_norm(const BlockNorm& a, const BlockNormOut& o, cudaStream_t stream) {
-  if (a.rows == 0) return LOOM_STATUS_OK;
+int launch_block_norm(const BlockNorm& a, const BlockNormOut& o, cudaStream_t stream) {
   const int w = a.width;
-  const bool by8 = rows_by_8(a.x, a.x_stride, w) && rows_by_8(a.h, a.h_stride, w) &&
-                   rows_by_8(a.gate, a.gate_stride, w) && rows_by_8(a.post_weight, w, w) &&
-                   rows_by_8(a.pre_weight, w, w) && rows_by_8(o.y, w, w) && rows_by_8(o.z, w, w);
-  const RowShape s = row_shape(w, by8);
-  const int64_t grid = s.warp ? ceil_div(a.rows, kRowWarps) : a.rows;
-  if (grid > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
-  return with_shape(s, [&](auto v, auto nv, auto warp) {
-    return launch_dependent(
-        block_norm_kernel<Tx, Tb, decltype(v)::value, decltype(nv)::value, decltype(warp)::value>,
-        dim3((unsigned)grid), s.block(), stream, a, o);
+  const bool row_gate = a.gate != nullptr && a.rows_per_gate == 1;
+  const bool phased = in_phase(a.x, a.x_stride, a.rows, w) && in_phase(a.h, a.h_stride, a.rows, w) &&
+                      (!row_gate || in_phase(a.gate, a.gate_stride, a.rows, w)) &&
+                      in_phase(o.y, w, a.rows, w) && in_phase(o.z, w, a.rows, w);
+  // two groups a thread and 512 threads an SM: with one group and twice the
+  // threads the registers spill (62 against 54 us for 8192 x 4096 bf16 rows).
+  // Where no row group has a second row, nothing is gained by staging.
+  RowPlan s = row_plan(w, phased, true, ForwardStage<Tx, Tb>::words, 512, 2, 128);
+  if (a.rows <= s.groups) s = row_plan(w, phased, false, 0, 1024, 1, 128);
+  s.groups = step_groups(s.groups, a.rows, w, s.phased);
+  if (a.gate != nullptr && !row_gate && s.groups < a.rows && a.rows_per_gate < s.groups) {
+    s.rows = ceil_div(a.rows, s.groups / 8 * 8);
+    s.groups = ceil_div(a.rows, 8 * s.rows) * 8;
+  }
+  return with_plan<2>(s, [&](auto staged, auto edge, auto per, auto warp, auto most) {
+    return launch_rows(block_norm_kernel<Tx, Tb, decltype(staged)::value, decltype(edge)::value,
+                                         decltype(per)::value, decltype(warp)::value,
+                                         decltype(most)::value>,
+                       s, stream, a, o);
   });
 }
 
-// The chunks of a backward pass: about one per row group, whole gate runs
-// where there are more runs than groups.
-inline int64_t grad_row_groups() { return (int64_t)kGradCtas * kRowWarps; }
+// Rows that a row group of the backward pass takes at least, where the SMs have
+// one group each: it leaves a partial row for them (777 x 1535 fp16 rows: 16.4 us
+// with 2, 17.6 with 4, 21 with 8).
+constexpr int kGroupRows = 2;
 
-inline int grad_chunks_per_gate(int64_t rows, int64_t gate_rows) {
-  if (gate_rows <= 0 || rows <= 0) return 1;
-  const int64_t run = rows / gate_rows;
-  int64_t c = grad_row_groups() / gate_rows;
-  if (c > run) c = run;
-  return c < 1 ? 1 : (int)c;
+// Row groups of the backward pass at most (partial rows of the workspace).
+inline int64_t grad_groups_most(int64_t rows, int64_t width) {
+  const int64_t most = width <= 1024 ? (int64_t)kSmCount * 8 : (int64_t)kSmCount * 2;
+  return rows < most ? rows : most;
 }
 
 inline size_t block_norm_grad_workspace_bytes(int64_t rows, int64_t width, int64_t gate_rows) {
   if (rows < 0 || width <= 0 || gate_rows < 0) return 0;
-  const int c = grad_chunks_per_gate(rows, gate_rows);
-  const int64_t lines = 2 * grad_row_groups() + (c > 1 ? gate_rows * c : 0);
-  return (size_t)lines * (size_t)align_up((size_t)width, 8) * sizeof(float) + 256;
+  const int64_t lines = grad_groups_most(rows, width) * (gate_rows > 0 ? 3 : 2);
+  return (size_t)lines * (size_t)width * sizeof(float) + 512;
 }
 
 template <class Tx, class Tb>
-inline int launch_block_norm_grad(const BlockNorm& a0, BlockNormGrad b, int64_t gate_rows,
+int launch_block_norm_grad(const BlockNorm& a0, BlockNormGrad b, int64_t gate_rows,
                                   void* dpost_weight, void* dpre_weight, void* workspace,
                                   cudaStream_t stream) {
   BlockNorm a = a0;
   const int w = a.width;
-  const bool by8 = rows_by_8(a.x, a.x_stride, w) && rows_by_8(a.h, a.h_stride, w) &&
-                   rows_by_8(a.gate, a.gate_stride, w) && rows_by_8(a.post_weight, w, w) &&
-                   rows_by_8(a.pre_weight, w, w) && rows_by_8(b.dy, b.dy_stride, w) &&
-                   rows_by_8(b.dz, b.dz_stride, w) && rows_by_8(b.dx, w, w) &&
-                   rows_by_8(b.dh, w, w) && rows_by_8(b.dgate, w, w);
-  const RowShape s = row_shape(w, by8);
-  const int64_t lanes = s.warp ? kRowWarps : 1;
-  const int64_t runs = a.gate != nullptr ? gate_rows : 1;
-  a.rows_per_gate = a.rows > 0 ? a.rows / runs : 1;
-  b.chunks_per_gate = grad_chunks_per_gate(a.rows, runs);
-  b.chunks = a.rows > 0 ? runs * b.chunks_per_gate : 0;
-  int64_t grid = ceil_div(b.chunks, lanes);
-  if (grid > kGradCtas) grid = kGradCtas;
-  const int64_t groups = grid * lanes;
-  float* rows = reinterpret_cast<float*>(workspace_base(workspace));
-  b.pre_rows = dpre_weight != nullptr ? rows : nullptr;
-  b.post_rows = dpost_weight != nullptr ? rows + grad_row_groups() * w : nullptr;
-  b.gate_rows = rows + 2 * grad_row_groups() * w;
-  if (grid > 0) {
-    const int st = with_shape(s, [&](auto v, auto nv, auto warp) {
-      return launch_dependent(block_norm_grad_kernel<Tx, Tb, decltype(v)::value,
-                                                     decltype(nv)::value, decltype(warp)::value>,
-                              dim3((unsigned)grid), s.block(), stream, a, b);
+  const int64_t rows = a.rows, most = grad_groups_most(rows, w);
+  a.rows_per_gate = a.gate != nullptr && rows > 0 ? rows / gate_rows : rows;
+  const bool row_gate = a.gate != nullptr && a.rows_per_gate == 1;
+  const int64_t runs = a.gate != nullptr && !row_gate ? gate_rows : 1;
+  b.run_rows = runs > 0 ? rows / runs : rows;
+  bool phased = in_phase(a.x, a.x_stride, rows, w) && in_phase(a.h, a.h_stride, rows, w) &&
+                (!row_gate || in_phase(a.gate, a.gate_stride, rows, w)) &&
+                in_phase(b.dy, b.dy_stride, rows, w) && in_phase(b.dz, b.dz_stride, rows, w) &&
+                in_phase(b.dx, w, rows, w) && in_phase(b.dh, w, rows, w) &&
+                (!row_gate || in_phase(b.dgate, w, rows, w));
+  // chunks of several runs have one phase where runs and chunks keep it
+  if (w % 8 != 0 && runs > 1 && (b.run_rows % 8 != 0 || 8 * runs > most)) phased = false;
+  RowPlan s = row_plan(w, phased, true, GradStage<Tx, Tb>::words, 512, 1, 64);
+  if (!(a.h != nullptr && b.dy != nullptr && a.pre_norm && a.post_norm)) s.edge = true;
+  int64_t groups = ceil_div(rows, (int64_t)kGroupRows);
+  if (groups < kSmCount) groups = kSmCount;
+  if (groups > s.groups) groups = s.groups;
+  if (groups > most) groups = most;
+  if (runs == 1) {
+    groups = step_groups(groups, rows, w, s.phased);
+    b.chunks_per_gate = (int)groups;
+    b.chunks = groups;
+  } else {
+    int64_t c = groups / runs;
+    if (s.phased && w % 8 != 0) c = c < 8 ? 8 : c / 8 * 8;
+    if (c > b.run_rows) c = b.run_rows;
+    b.chunks_per_gate = (int)(c < 1 ? 1 : c);
+    b.chunks = runs * b.chunks_per_gate;
+    groups = step_groups(groups, b.chunks, w, s.phased);
+  }
+  s.groups = groups;
+  float* partial = reinterpret_cast<float*>(workspace_base(workspace));
+  b.pre_rows = dpre_weight != nullptr ? partial : nullptr;
+  b.post_rows = dpost_weight != nullptr ? partial + most * w : nullptr;
+  b.gate_rows = partial + 2 * most * w;
+  if (rows > 0) {
+    const bool whole = a.h != nullptr && b.dy != nullptr && a.pre_norm && a.post_norm;
+    const int st = with_plan<1>(s, [&](auto staged, auto edge, auto per, auto warp, auto most) {
+      auto launch = [&](auto gate, auto all) {
+        return launch_rows(
+            block_norm_grad_kernel<Tx, Tb, decltype(staged)::value, decltype(edge)::value,
+                                   decltype(per)::value, decltype(warp)::value,
+                                   decltype(most)::value, (Gate)decltype(gate)::value,
+                                   decltype(all)::value>,
+            s, stream, a, b);
+      };
+      auto by_gate = [&](auto all) {
+        return a.gate == nullptr ? launch(std::integral_constant<int, kNoGate>(), all)
+               : row_gate        ? launch(std::integral_constant<int, kRowGate>(), all)
+                                 : launch(std::integral_constant<int, kRunGate>(), all);
+      };
+      if constexpr (decltype(staged)::value)
+        if (whole) return by_gate(std::true_type());
+      if constexpr (decltype(edge)::value) return by_gate(std::false_type());
+      return (int)LOOM_STATUS_CUDA_ERROR;
     });
     if (st != LOOM_STATUS_OK) return st;
   }
   RowSums sums;
-  sums.rows[0] = rows;
-  sums.rows[1] = rows + grad_row_groups() * w;
+  sums.rows[0] = partial;
+  sums.rows[1] = partial + most * w;
   sums.rows[2] = b.gate_rows;
   sums.out[0] = dpre_weight;
   sums.out[1] = dpost_weight;
   sums.out[2] = b.dgate;
-  sums.groups = groups;
+  sums.groups = rows > 0 ? groups : 0;
   sums.chunks_per_gate = b.chunks_per_gate;
   sums.width = w;
-  const bool gate_jobs = b.dgate != nullptr && (b.chunks_per_gate > 1);
+  const bool gate_jobs = b.dgate != nullptr && !row_gate && b.chunks_per_gate > 1;
   const bool weights = dpre_weight != nullptr || dpost_weight != nullptr;
   const int first = weights ? 0 : 2;
   const int64_t jobs = (weights ? 2 : 0) + (gate_jobs ? runs : 0);
   if (jobs == 0) return LOOM_STATUS_OK;
   return launch_dependent(block_norm_sums_kernel<Tb>,
-                          dim3((unsigned)ceil_div(w, 32), (unsigned)jobs), dim3(256), stream, sums,
-                          first);
+                          dim3((unsigned)ceil_div(w, 32), (unsigned)jobs), dim3(256), stream,
+                          (size_t)0, sums, first);
 }
+
+// The pairs of a residual stream's and a branch's element types.  Each pair and
+// direction is compiled on its own (b200_train_rows.cu).
+#define LOOM_ROW_TYPES(X)          \
+  X(float, float)                  \
+  X(float, __nv_bfloat16)          \
+  X(float, __half)                 \
+  X(__nv_bfloat16, __nv_bfloat16)  \
+  X(__half, __half)
 
 }  // namespace loomb

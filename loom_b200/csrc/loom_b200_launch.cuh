@@ -183,14 +183,15 @@ inline void launch_pdl(Kern kernel, unsigned grid, cudaStream_t stream, Args... 
   kernel<<<grid, kThreads, 0, stream>>>(args...);
 }
 
-// The same launch with any grid and block; returns a status.
+// The same launch with any grid, block and bytes of dynamic shared memory;
+// returns a status.
 template <class Kern, class... Args>
 inline int launch_dependent(Kern kernel, dim3 grid, dim3 block, cudaStream_t stream,
-                            const Args&... args) {
+                            size_t shared, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
-  cfg.dynamicSmemBytes = 0;
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

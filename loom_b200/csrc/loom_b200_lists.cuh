@@ -189,12 +189,12 @@ inline int launch_list_norm_parts(int64_t count, const void* const* grads, const
     t.tiles = (uint32_t)tiles;
     const unsigned grid = clamp_grid(tiles, kNormMaxCtas);
     const int st = launch_dependent(list_norm_kernel<T, kCap>, dim3(grid), dim3(kThreads),
-                                    stream, t, partials + filled);
+                                    stream, (size_t)0, t, partials + filled);
     if (st != LOOM_STATUS_OK) return st;
     filled += (int)grid;
   }
   return launch_dependent(list_norm_finalize_kernel, dim3(1), dim3(kFinalizeThreads), stream,
-                          (const double*)partials, filled, max_norm, out);
+                          (size_t)0, (const double*)partials, filled, max_norm, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -426,12 +426,6 @@ struct Adam8Table {
   int warp_blocks;             // consecutive blocks that each warp takes
 };
 
-// Eight consecutive elements as they lie in memory.
-template <class T>
-struct Raw8 {
-  uint4 word[sizeof(T) / 2];
-};
-
 // Eight consecutive elements of which the first `left` exist; the others are
 // zero.
 template <class T>
@@ -450,17 +444,6 @@ __device__ __forceinline__ void load8_some(Raw8<T>& r, const T* p, int left) {
 #pragma unroll
   for (int k = 0; k < (int)sizeof(T) / 2; ++k)
     r.word[k] = make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
-}
-template <class T>
-__device__ __forceinline__ F2 pair_of(const Raw8<T>& r, int j) {
-  const unsigned* u = reinterpret_cast<const unsigned*>(r.word);
-  if constexpr (sizeof(T) == 4) {
-    return f2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
-  } else {
-    float a, b;
-    widen2(a, b, u[j], T());
-    return f2(a, b);
-  }
 }
 template <class T>
 __device__ __forceinline__ void store8_some(T* p, const float (&f)[8], int left) {
@@ -536,27 +519,7 @@ __device__ __forceinline__ float largest(float a, float b, float c) {
   return r;
 }
 
-// One lane's part of a block on its way through shared memory.  A lane copies
-// what it reads itself (cp.async), so that its own wait is all that is needed
-// between the two.
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                   (unsigned)__cvta_generic_to_shared(to)),
-               "l"(from)
-               : "memory");
-}
-__device__ __forceinline__ void copy8(void* to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
-                   (unsigned)__cvta_generic_to_shared(to)),
-               "l"(from)
-               : "memory");
-}
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLater>
-__device__ __forceinline__ void wait_copies() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory");
-}
-
+// One lane's part of a block on its way through shared memory.
 template <class Tw, class Tg>
 struct BlockStage {
   uint4 w[sizeof(Tw) / 2][kThreads];
@@ -839,7 +802,7 @@ inline int launch_adamw_parts(const AdamLists& l, const StepConst& c, const Step
     }
     if (t.count == 0) break;
     const int st = launch_dependent(adamw_kernel<Tp, Tg, kMaster, kCap>, dim3((unsigned)tiles),
-                                    dim3(kThreads), stream, t, values, c);
+                                    dim3(kThreads), stream, (size_t)0, t, values, c);
     if (st != LOOM_STATUS_OK) return st;
   }
   return LOOM_STATUS_OK;
@@ -881,7 +844,7 @@ inline int launch_adamw8_parts(const AdamLists& l, const StepConst& c, const Ste
     }
     if (t.count == 0) break;
     const int st = launch_dependent(adamw8_kernel<Tp, Tg, kMaster, kCap>, dim3((unsigned)tiles),
-                                    dim3(kThreads), stream, t, values, c);
+                                    dim3(kThreads), stream, (size_t)0, t, values, c);
     if (st != LOOM_STATUS_OK) return st;
   }
   return LOOM_STATUS_OK;

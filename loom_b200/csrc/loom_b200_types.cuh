@@ -200,4 +200,49 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
+// Eight consecutive elements as they lie in memory.
+template <class T>
+struct Raw8 {
+  uint4 word[sizeof(T) / 2];
+};
+
+template <class T>
+__device__ __forceinline__ F2 pair_of(const Raw8<T>& r, int j) {
+  const unsigned* u = reinterpret_cast<const unsigned*>(r.word);
+  if constexpr (sizeof(T) == 4) {
+    return f2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+  } else {
+    float a, b;
+    widen2(a, b, u[j], T());
+    return f2(a, b);
+  }
+}
+// Asynchronous copies to shared memory.  Every user here lets a thread copy
+// what the same thread reads, so that its own wait is all that is needed
+// between the two.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(to)),
+               "l"(from)
+               : "memory");
+}
+// The first `bytes` of 16; the rest become zeros and are not read.
+__device__ __forceinline__ void copy16_some(void* to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(to)),
+               "l"(from), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void copy8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(
+                   (unsigned)__cvta_generic_to_shared(to)),
+               "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLater>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory");
+}
+
 }  // namespace loomb

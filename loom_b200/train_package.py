@@ -16,13 +16,28 @@ import shlex
 import shutil
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
-from typing import List
+from typing import List, Tuple
 
 from .artifact import (CSRC, CUDA_ARCH, GENCODE, BuildError, PackageResult, _run, _write)
 
 PACKAGE = "b200_train"
 HEADER = Path(__file__).resolve().parent.parent / "include" / "loom" / f"{PACKAGE}.h"
-SOURCES = ("b200_train_lists.cu", "b200_train_norms.cu")
+SOURCES = ("b200_train_lists.cu", "b200_train_norms.cu", "b200_train_rows.cu")
+
+# the element types of block_norm's residual stream and branch
+ROW_TYPES = (("float", "float"), ("float", "__nv_bfloat16"), ("float", "__half"),
+             ("__nv_bfloat16", "__nv_bfloat16"), ("__half", "__half"))
+
+
+def _units() -> List[Tuple[str, str, List[str]]]:
+    """(source, object, defines) of every compilation."""
+    units = [(s, s[:-3] + ".o", []) for s in SOURCES[:2]]
+    for x, b in ROW_TYPES:
+        for backward in (0, 1):
+            obj = f"rows_{x.strip('_')}_{b.strip('_')}_{'backward' if backward else 'forward'}.o"
+            units.append((SOURCES[2], obj, [f"-DLOOM_ROWS_X={x}", f"-DLOOM_ROWS_B={b}",
+                                            f"-DLOOM_ROWS_BACKWARD={backward}"]))
+    return units
 
 # entry name -> (what it does, whether it takes a workspace)
 ENTRIES = {
@@ -43,9 +58,9 @@ def _commands(nvcc: str, include_dir: str, out_dir: str, artifact: str, kind: st
     base = [nvcc, "-std=c++17", "-O3", "-gencode", GENCODE, "-fmad=false", "-lineinfo",
             "-Xptxas", "-O3", f"-I{include_dir}", f"-I{CSRC}", "-c", "-Xcompiler", "-fPIC"]
     compiles, objects = [], []
-    for name in SOURCES:
-        obj = os.path.join(out_dir, "src-gen", name[:-3] + ".o")
-        compiles.append(base + ["-o", obj, str(CSRC / name)])
+    for name, obj, defines in _units():
+        obj = os.path.join(out_dir, "src-gen", obj)
+        compiles.append(base + defines + ["-o", obj, str(CSRC / name)])
         objects.append(obj)
     if kind == "shared":
         return compiles, [[nvcc, "-shared", "-gencode", GENCODE, "-o", artifact] + objects]
@@ -77,7 +92,7 @@ def generate_train_package(out_dir: str, kind: str = "shared", nvcc: str = "nvcc
         if shutil.which(nvcc) is None and not os.path.exists(nvcc):
             raise BuildError("nvcc is required on PATH for the Loom B200 backend")
         os.makedirs(os.path.join(out_dir, "src-gen"), exist_ok=True)
-        with ThreadPoolExecutor(len(compiles)) as pool:
+        with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
             list(pool.map(_run, compiles))
         if kind == "static" and os.path.exists(artifact):
             os.remove(artifact)
