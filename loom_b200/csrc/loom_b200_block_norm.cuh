@@ -165,8 +165,8 @@ __device__ __forceinline__ F2 dot8(const Group& a, const Group& b, F2 sum) {
   return sum;
 }
 
-// kEdge false: each thread's groups lie wholly in the row.  True: the first and
-// the last group may be partly outside, and threads may be left over.
+// kEdge false: each group lies wholly in the row (and in the staged kernels no
+// thread is left over).  True: the first and the last group may be partly outside.
 template <bool kEdge>
 __device__ __forceinline__ bool inside(int e, int width) {
   return !kEdge || (e >= 0 && e + 8 <= width);
@@ -193,15 +193,17 @@ __device__ __forceinline__ Group within(Group g, int e, int width) {
   return g;
 }
 // The group of a row that begins `e` elements after the row's start (which may
-// be before it), from any place; zero outside the row.
-template <class T>
+// be before it), zero outside the row.  kAny: from any place, else each group is
+// wholly inside or outside and at a 16-byte boundary.
+template <bool kAny = true, class T>
 __device__ __forceinline__ Group load_group(const T* row, int e, int width) {
   float f[8];
-  if (e >= 0 && e + 8 <= width && ((uintptr_t)(row + e) & 15u) == 0) {
+  if (kAny ? e >= 0 && e + 8 <= width && ((uintptr_t)(row + e) & 15u) == 0 : e < width) {
     load_vec<8, kKeep>(f, row + e);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = e + i >= 0 && e + i < width ? widen(row[e + i]) : 0.0f;
+    for (int i = 0; i < 8; ++i)
+      f[i] = kAny && e + i >= 0 && e + i < width ? widen(row[e + i]) : 0.0f;
   }
   Group g;
 #pragma unroll
@@ -284,6 +286,12 @@ __device__ __forceinline__ Raw8<T> read_raw(const uint4* slot, int pitch) {
   return r;
 }
 
+template <class T>
+__device__ __forceinline__ void store_raw(uint4* slot, int pitch, const Raw8<T>& r) {
+#pragma unroll
+  for (int k = 0; k < GroupWords<T>::value; ++k) slot[k * pitch] = r.word[k];
+}
+
 __device__ __forceinline__ void wait_stage(int stages) {
   if (stages == 4) {
     wait_copies<2>();
@@ -336,7 +344,7 @@ struct ForwardStage {
 };
 
 template <class Tx, class Tb, bool kStaged, bool kEdge, int NV, bool kWarp, int kMost>
-__global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1)
+__global__ void __launch_bounds__(kMost, kStaged ? (kMost == 256 ? 2 : 1) : kWarp ? 8 : 1024 / kMost)
 block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
@@ -358,7 +366,7 @@ block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     e[j] = (j * threads + (int)threadIdx.x) * 8 - phase;
-    any[j] = !kEdge || e[j] < width;
+    any[j] = (kStaged && !kEdge) || e[j] < width;
   }
   uint4* const mine = slots + threadIdx.y * threads + threadIdx.x;
   auto slot = [&](int stage, int j, int part) {
@@ -412,9 +420,10 @@ block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!kStaged) {
-        y[j] = load_group(row_at<Tx>(a.x, row, a.x_stride), e[j], width);
-        if (has_h) u[j] = load_group(row_at<Tb>(a.h, row, a.h_stride), e[j], width);
-        if (row_gate) gate[j] = load_group(row_at<Tb>(a.gate, row, a.gate_stride), e[j], width);
+        y[j] = load_group<kEdge>(row_at<Tx>(a.x, row, a.x_stride), e[j], width);
+        if (has_h) u[j] = load_group<kEdge>(row_at<Tb>(a.h, row, a.h_stride), e[j], width);
+        if (row_gate)
+          gate[j] = load_group<kEdge>(row_at<Tb>(a.gate, row, a.gate_stride), e[j], width);
       } else if (any[j]) {
         y[j] = within<kEdge>(unpack(read_raw<Tx>(slot(stage, j, Stage::x), pitch)), e[j], width);
         if (has_h)
@@ -444,7 +453,7 @@ block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
       for (int j = 0; j < NV; ++j) {
         y[j] = fma8(u[j] * rstd * w_post[j] * gate[j], a.branch_scale, y[j] * a.residual_scale);
         if (any[j])
-          store_group<kStaged, kEdge>(row_at<Tx>(o.y, row, width), y[j], e[j], width);
+          store_group<kStaged || !kEdge, kEdge>(row_at<Tx>(o.y, row, width), y[j], e[j], width);
       }
     }
     if (!a.pre_norm) continue;
@@ -456,8 +465,8 @@ block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (any[j])
-        store_group<kStaged, kEdge>(row_at<Tb>(o.z, row, width), y[j] * rstd * w_pre[j], e[j],
-                                    width);
+        store_group<kStaged || !kEdge, kEdge>(row_at<Tb>(o.z, row, width),
+                                              y[j] * rstd * w_pre[j], e[j], width);
   }
   if (kStaged) wait_copies<0>();
 }
@@ -537,7 +546,7 @@ enum Gate : int { kNoGate = 0, kRowGate = 1, kRunGate = 2 };
 // of the instructions: 103 against 119 us for 8192 x 4096 bf16 rows).
 template <class Tx, class Tb, bool kStaged, bool kEdge, int NV, bool kWarp, int kMost, Gate kGate,
           bool kWhole>
-__global__ void __launch_bounds__(kMost)
+__global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1)
 block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan plan) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
@@ -553,6 +562,8 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
   const int phase = kEdge && plan.phased ? (int)((group * width) & 7) : 0;
   const int pitch = threads * blockDim.y;
   const bool has_h = kWhole || a.h != nullptr, has_dy = kWhole || b.dy != nullptr;
+  const float post_offset = a.post_weight != nullptr ? a.offset : 0.0f;
+  const float pre_offset = a.pre_weight != nullptr ? a.offset : 0.0f;
   const bool pre_norm = kWhole || a.pre_norm, post_norm = kWhole || (a.post_norm && has_h);
 
   int e[NV];
@@ -606,11 +617,37 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
     ahead.next(b, groups);
   }
   Raw8<Tb> gate[NV];
-  Group w_post[NV], w_pre[NV], s_pre[NV], s_post[NV], s_gate[NV];
+  Group s_pre[NV], s_post[NV], s_gate[NV];
+  // Where registers are short (two groups a thread, or 1024 threads) the weights
+  // stay in shared memory, each thread's own beside its stages, or where they are.
+  constexpr bool kHold = kStaged && NV == 1 && kMost < 1024;
+  Group held[kHold ? 2 : 1];
+  auto weight_slot = [&](int j, int part) {
+    return mine + ((stages * NV * Stage::words) + (j * 2 + part) * GroupWords<Tb>::value) * pitch;
+  };
+  auto weight = [&](int j, int part) {
+    if (kHold) return held[kHold ? part : 0];
+    if (!kStaged)
+      return load_weight(static_cast<const Tb*>(part ? a.post_weight : a.pre_weight), a.offset,
+                         e[j], width);
+    const float offset = part ? post_offset : pre_offset;
+    Group w = unpack(read_raw<Tb>(weight_slot(j, part), pitch));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.p[i] = add2(w.p[i], f2(offset, offset));
+    return w;
+  };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    w_post[j] = load_weight(static_cast<const Tb*>(a.post_weight), a.offset, e[j], width);
-    w_pre[j] = load_weight(static_cast<const Tb*>(a.pre_weight), a.offset, e[j], width);
+    if (kHold) {
+      held[0] = load_weight(static_cast<const Tb*>(a.pre_weight), a.offset, e[j], width);
+      held[kHold ? 1 : 0] =
+          load_weight(static_cast<const Tb*>(a.post_weight), a.offset, e[j], width);
+    } else if (kStaged) {
+      store_raw(weight_slot(j, 0), pitch,
+                load_raw(static_cast<const Tb*>(a.pre_weight), e[j], width));
+      store_raw(weight_slot(j, 1), pitch,
+                load_raw(static_cast<const Tb*>(a.post_weight), e[j], width));
+    }
     gate[j] = load_raw(static_cast<const Tb*>(nullptr), e[j], width);
     s_pre[j] = s_post[j] = s_gate[j] = same(0.0f);
   }
@@ -647,7 +684,7 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
         n[j] = fetch(Tx(), a.x, row, a.x_stride, stage, j, Stage::y) * pre_rstd;
         Group t = fetch(Tb(), b.dz, row, b.dz_stride, stage, j, Stage::dz);
         s_pre[j] = fma8(t, n[j], s_pre[j]);
-        t = t * w_pre[j];
+        t = t * weight(j, 0);
         tn = dot8(t, n[j], tn);
         f[j] = fma8(t, pre_rstd, f[j]);
       }
@@ -658,7 +695,7 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
           else if (any[j]) gate[j] = read_raw<Tb>(slot(stage, j, Stage::gate), pitch);
         }
         if (post_norm) {
-          Group c = w_post[j] * k[j];
+          Group c = weight(j, 1) * k[j];
           if (kGate != kNoGate) c = c * within<kEdge>(unpack(gate[j]), e[j], width);
           cfk = dot8(c, f[j], cfk);
           cnk = dot8(c, n[j], cnk);
@@ -679,6 +716,7 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
                                     width);
       if (has_h) {
         const Group scaled = d * a.branch_scale, own = scaled * k[j];
+        const Group w = weight(j, 1);
         Group through = scaled, sum = own;  // with the gate
         if (kGate != kNoGate) {
           const Group g = within<kEdge>(unpack(gate[j]), e[j], width);
@@ -687,12 +725,12 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
         }
         if (kGate == kRowGate) {
           if (any[j])
-            store_group<kStaged, kEdge>(row_at<Tb>(b.dgate, row, width), own * w_post[j], e[j], width);
+            store_group<kStaged, kEdge>(row_at<Tb>(b.dgate, row, width), own * w, e[j], width);
         } else if (kGate == kRunGate) {
-          s_gate[j] = fma8(own, w_post[j], s_gate[j]);
+          s_gate[j] = fma8(own, w, s_gate[j]);
         }
         s_post[j] = s_post[j] + sum;
-        const Group dh = fma8(k[j], post_pull, through * w_post[j]) * post_rstd;
+        const Group dh = fma8(k[j], post_pull, through * w) * post_rstd;
         if (any[j])
           store_group<kStaged, kEdge>(row_at<Tb>(b.dh, row, width), dh, e[j], width);
       }
@@ -776,19 +814,19 @@ inline bool in_phase(const void* p, int64_t stride, int64_t rows, int width) {
                           (rows <= 1 || (stride >= width && (stride - width) % 8 == 0)));
 }
 
-// `words`: 16-byte words of a stage per thread and group of eight; `per`: groups
+// `words`, `fixed`: 16-byte words per thread and group of eight, of a stage and
+// beside the stages; `per`: groups
 // per thread of a staged CTA; `resident`: threads per SM that the kernel's
-// registers allow, about; `warp_units`: groups of eight that a warp takes at
-// most.  `stage`: whether rows come through stages at all.
-inline RowPlan row_plan(int width, bool phased, bool stage, int words, int resident, int per,
-                        int warp_units) {
+// registers allow, about.  `stage`: whether rows come through stages at all.
+inline RowPlan row_plan(int width, bool phased, bool stage, int words, int fixed, int resident,
+                        int per, bool backward) {
   RowPlan s = {};
   s.phased = phased;
   const int units = phased && width % 8 != 0 ? (width + 14) / 8 : (width + 7) / 8;
   for (int staged = phased && stage ? 1 : 0;; --staged) {
-    s.warp = units <= warp_units;
+    s.warp = units <= 32;
     if (s.warp) {
-      s.per = units <= 32 ? 1 : units <= 64 ? 2 : 4;
+      s.per = 1;
       s.threads = 32;
       s.most = 32 * kRowWarps;
     } else {
@@ -804,19 +842,24 @@ inline RowPlan row_plan(int width, bool phased, bool stage, int words, int resid
     const int threads = (int)s.threads * (s.warp ? kRowWarps : 1);
     int ctas = resident / threads;
     if (ctas < 1) ctas = 1;
-    s.edge = !staged || width % 8 != 0 || units != (int)s.threads * s.per;
+    // weights beside the stages: see kHold
+    const size_t held = staged && (s.per > 1 || s.most == 1024) ? (size_t)s.per * fixed * 16 * threads : 0;
+    s.edge = width % 8 != 0 || (staged ? units != (int)s.threads * s.per : !phased || backward);
     if (staged) {
       const size_t bytes = (size_t)s.per * words * 16 * threads;
       // wider than the staged kernels go, or than shared memory holds two rows of
-      if (threads > s.most || 2 * bytes > kStageBytes) continue;
-      if (2 * bytes * ctas > kStageBytes) ctas = (int)(kStageBytes / (2 * bytes));
-      const size_t fit = kStageBytes / ctas / bytes;
+      if (threads > s.most || (per == 2 && backward && s.most == 1024) ||
+          2 * bytes + held > kStageBytes)
+        continue;
+      if ((2 * bytes + held) * ctas > kStageBytes) ctas = (int)(kStageBytes / (2 * bytes + held));
+      const size_t fit = (kStageBytes / ctas - held) / bytes;
       s.stages = fit < 4 ? (int)fit : 4;
       s.shared = (size_t)s.stages * bytes;
     } else if (units > 4096) {
       // an odd width whose shifted groups pass the widest CTA: unshifted
-      return row_plan(width, false, false, words, resident, per, warp_units);
+      return row_plan(width, false, false, words, fixed, resident, per, backward);
     }
+    s.shared += held;
     s.groups = (int64_t)kSmCount * ctas * (s.warp ? kRowWarps : 1);
     return s;
   }
@@ -841,9 +884,8 @@ inline int launch_rows(Kern kernel, const RowPlan& s, cudaStream_t stream, const
   return launch_dependent(kernel, s.grid(), s.block(), stream, s.shared, args..., s);
 }
 
-// Calls f with the plan as constants; kPer 2 is the forward pass's, 1 the
-// backward's, whose warps take at most two groups a lane.
-template <int kPer, class F>
+// Calls f with the plan as constants.
+template <bool kBackward, class F>
 inline int with_plan(const RowPlan& s, const F& f) {
   using std::integral_constant;
   const std::true_type yes;
@@ -852,27 +894,26 @@ inline int with_plan(const RowPlan& s, const F& f) {
   const integral_constant<int, 2> two;
   const integral_constant<int, 4> four;
   const integral_constant<int, 32 * kRowWarps> warps;
+  const integral_constant<int, 256> quarter;
   const integral_constant<int, 512> half;
   const integral_constant<int, 1024> full;
-  auto by_warps = [&](auto staged, auto edge) {
-    if constexpr (kPer > 1)
-      if (s.per == 4) return f(staged, edge, four, yes, warps);
-    return s.per == 1 ? f(staged, edge, one, yes, warps) : f(staged, edge, two, yes, warps);
-  };
   if (s.stages == 0) {
-    if (s.warp) return by_warps(no, yes);
     if (s.per == 4) return f(no, yes, four, no, full);
-    return s.most == 512 ? f(no, yes, one, no, half) : f(no, yes, one, no, full);
+    auto direct = [&](auto edge) {
+      return s.warp          ? f(no, edge, one, yes, warps)
+             : s.most == 512 ? f(no, edge, one, no, half)
+                             : f(no, edge, one, no, full);
+    };
+    if constexpr (!kBackward)
+      if (!s.edge) return direct(no);
+    return direct(yes);
   }
   auto staged = [&](auto edge) {
-    if (s.warp) return by_warps(yes, edge);
-    const integral_constant<int, kPer> per;
-    const integral_constant<int, 512 / kPer> narrow_cta;
-    const integral_constant<int, 1024 / kPer> wide_cta;
-    if (s.most == 512 / kPer) return f(yes, edge, per, no, narrow_cta);
-    if (s.most == 1024 / kPer) return f(yes, edge, per, no, wide_cta);
-    if constexpr (kPer > 1) return f(yes, edge, per, no, full);
-    return (int)LOOM_STATUS_CUDA_ERROR;
+    if (s.warp) return f(yes, edge, one, yes, warps);
+    if (s.per == 2 && s.most == 256) return f(yes, edge, two, no, quarter);
+    if (s.per == 2 && s.most == 512) return f(yes, edge, two, no, half);
+    if constexpr (kBackward) return s.most == 512 ? f(yes, edge, one, no, half) : f(yes, edge, one, no, full);
+    return f(yes, edge, two, no, full);
   };
   return s.edge ? staged(yes) : staged(no);
 }
@@ -886,15 +927,21 @@ int launch_block_norm(const BlockNorm& a, const BlockNormOut& o, cudaStream_t st
                       in_phase(o.y, w, a.rows, w) && in_phase(o.z, w, a.rows, w);
   // two groups a thread and 512 threads an SM: with one group and twice the
   // threads the registers spill (62 against 54 us for 8192 x 4096 bf16 rows).
-  // Where no row group has a second row, nothing is gained by staging.
-  RowPlan s = row_plan(w, phased, true, ForwardStage<Tx, Tb>::words, 512, 2, 128);
-  if (a.rows <= s.groups) s = row_plan(w, phased, false, 0, 1024, 1, 128);
+  // Where there are hardly more rows than row groups, nothing is gained by
+  // staging: every row has a CTA or a warp of its own.
+  RowPlan s = row_plan(w, phased, true, ForwardStage<Tx, Tb>::words, 0, 512, 2, false);
+  // (1533 rows of 1024, fp32 beside bf16: 6.3 against 7.9 us; of 1040, which leave
+  // threads over, 7.0 against 9.4; but 3000 bf16 rows of 1024 8.9 against 7.3.)
+  if (s.stages == 0 || a.rows <= (w > 1088 ? 1 : s.edge ? 3 : 2) * s.groups) {
+    s = row_plan(w, phased, false, 0, 0, 1024, 1, false);
+    s.groups = a.rows;
+  }
   s.groups = step_groups(s.groups, a.rows, w, s.phased);
   if (a.gate != nullptr && !row_gate && s.groups < a.rows && a.rows_per_gate < s.groups) {
     s.rows = ceil_div(a.rows, s.groups / 8 * 8);
     s.groups = ceil_div(a.rows, 8 * s.rows) * 8;
   }
-  return with_plan<2>(s, [&](auto staged, auto edge, auto per, auto warp, auto most) {
+  return with_plan<false>(s, [&](auto staged, auto edge, auto per, auto warp, auto most) {
     return launch_rows(block_norm_kernel<Tx, Tb, decltype(staged)::value, decltype(edge)::value,
                                          decltype(per)::value, decltype(warp)::value,
                                          decltype(most)::value>,
@@ -937,7 +984,14 @@ int launch_block_norm_grad(const BlockNorm& a0, BlockNormGrad b, int64_t gate_ro
                 (!row_gate || in_phase(b.dgate, w, rows, w));
   // chunks of several runs have one phase where runs and chunks keep it
   if (w % 8 != 0 && runs > 1 && (b.run_rows % 8 != 0 || 8 * runs > most)) phased = false;
-  RowPlan s = row_plan(w, phased, true, GradStage<Tx, Tb>::words, 512, 1, 64);
+  // Two groups a thread and 256 threads: two CTAs share an SM and cover each
+  // other's barriers (8192 x 4096 bf16 rows: 95 against 105 us); with edges or a
+  // gate row's sums beside, the registers spill (25 against 16 us for 777 x 1535
+  // fp16 rows), and few or narrow rows gain nothing (2048 wide: 53 against 47).
+  const bool run_gate = a.gate != nullptr && !row_gate;
+  const bool two = w % 8 == 0 && !run_gate && (w > 4096 || (w > 2048 && rows >= 2048));
+  RowPlan s = row_plan(w, phased, true, GradStage<Tx, Tb>::words, 2 * GroupWords<Tb>::value, 512,
+                       two ? 2 : 1, true);
   if (!(a.h != nullptr && b.dy != nullptr && a.pre_norm && a.post_norm)) s.edge = true;
   int64_t groups = ceil_div(rows, (int64_t)kGroupRows);
   if (groups < kSmCount) groups = kSmCount;
@@ -962,7 +1016,7 @@ int launch_block_norm_grad(const BlockNorm& a0, BlockNormGrad b, int64_t gate_ro
   b.gate_rows = partial + 2 * most * w;
   if (rows > 0) {
     const bool whole = a.h != nullptr && b.dy != nullptr && a.pre_norm && a.post_norm;
-    const int st = with_plan<1>(s, [&](auto staged, auto edge, auto per, auto warp, auto most) {
+    const int st = with_plan<true>(s, [&](auto staged, auto edge, auto per, auto warp, auto most) {
       auto launch = [&](auto gate, auto all) {
         return launch_rows(
             block_norm_grad_kernel<Tx, Tb, decltype(staged)::value, decltype(edge)::value,
