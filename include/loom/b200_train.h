@@ -47,7 +47,8 @@ int loom_train_adamw_stream(int64_t count, void* const* params, const void* cons
 /* adamw8: the same step with both moments in 8 bits.  Blocks of 256 values of a tensor (the last one may be short) share an fp32 top, the block's largest magnitude;
    a value is e4m3 code * top / 256.  exp_avg_top[i] and exp_avg_sq_top[i] hold ceil(sizes[i] / 256) tops.  The step computes in fp32 and rounds each new moment up or down
    with the probability of its distance, by random bits of (seed, t, place in the list); a second moment above zero never becomes zero.  A block with a moment that is not
-   finite reads back as not finite throughout; one whose largest is below 2^-100 holds zeros.  eps > 0. */
+   finite reads back as not finite throughout; one whose largest is below 2^-100 holds zeros.
+   The sign of a code that stands for zero is not specified.  eps is at least FLT_MIN. */
 size_t loom_train_adamw8_workspace_size(int64_t count);
 int loom_train_adamw8(int64_t count, void* const* params, const void* const* grads, uint8_t* const* exp_avg, uint8_t* const* exp_avg_sq, float* const* exp_avg_top, float* const* exp_avg_sq_top, float* const* master, const int64_t* sizes, const double* weight_decay, int param_dtype, int grad_dtype, const float* lr, double beta1, double beta2, double eps, const float* grad_scale, int64_t* step, uint64_t seed, void* workspace, size_t workspace_size);
 int loom_train_adamw8_stream(int64_t count, void* const* params, const void* const* grads, uint8_t* const* exp_avg, uint8_t* const* exp_avg_sq, float* const* exp_avg_top, float* const* exp_avg_sq_top, float* const* master, const int64_t* sizes, const double* weight_decay, int param_dtype, int grad_dtype, const float* lr, double beta1, double beta2, double eps, const float* grad_scale, int64_t* step, uint64_t seed, void* workspace, size_t workspace_size, void* stream);
@@ -56,7 +57,7 @@ int loom_train_adamw8_stream(int64_t count, void* const* params, const void* con
      u = h post_rstd (post_weight + weight_offset), post_rstd = 1 / sqrt(mean(h^2) + eps)   (post_norm 0: u = h)
      y = residual_scale x + branch_scale gate u
      z = y pre_rstd (pre_weight + weight_offset), pre_rstd = 1 / sqrt(mean(y^2) + eps)      (pre_norm 0: no z)
-   x, y are of x_dtype; h, gate, the weights and z of h_dtype (x_dtype, or 16-bit beside a 32-bit x).  h null: y is x, is not written and may be null.
+   x, y are of x_dtype; h, gate, the weights and z of h_dtype (x_dtype, or 16-bit beside a 32-bit x).  rows and strides are below 2^31.  h null: y is x, is not written and may be null.
    gate (or null): gate_rows rows, each for rows / gate_rows consecutive rows.  A null weight is all ones (no offset).  Strides are in elements, outputs contiguous;
    post_rstd and pre_rstd ([rows], for the backward pass) may be null. */
 int loom_train_block_norm(const void* x, int64_t x_stride, const void* h, int64_t h_stride, const void* gate, int64_t gate_stride, int64_t gate_rows, const void* post_weight, const void* pre_weight, int64_t rows, int64_t width, int x_dtype, int h_dtype, int post_norm, int pre_norm, float eps, float weight_offset, float residual_scale, float branch_scale, void* y, void* z, float* post_rstd, float* pre_rstd);

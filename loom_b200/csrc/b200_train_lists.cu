@@ -1,6 +1,8 @@
 // C entries of the operators over lists of tensors (include/loom/b200_train.h):
 // argument checks, the choice of the kernel by the element types, launches.
 // Build: -gencode arch=compute_100a,code=sm_100a -fmad=false.
+#include <float.h>
+
 #include "loom/b200_train.h"
 
 #include "loom_b200_lists.cuh"
@@ -82,7 +84,7 @@ int adamw_impl(const AdamLists& l, int param_dtype, int grad_dtype, const float*
   if (!sizes_ok(l.count, l.sizes) || !loomb::valid_dtype(param_dtype) ||
       !loomb::valid_dtype(grad_dtype) || !(beta1 >= 0.0 && beta1 < 1.0) ||
       !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0 && eps < (double)INFINITY) ||
-      (kEight && (float)eps == 0.0f) || lr == nullptr || !aligned_to(lr, 4) ||
+      (kEight && !((float)eps >= FLT_MIN)) || lr == nullptr || !aligned_to(lr, 4) ||
       !aligned_to(grad_scale, 4) || step == nullptr || !aligned_to(step, 8))
     return LOOM_STATUS_INVALID_ARGUMENT;
   if (!list_ok(l.count, l.params, l.sizes, loomb::dtype_bytes(param_dtype)) ||

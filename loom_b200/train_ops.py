@@ -29,7 +29,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 from .loader import LoomError, _torch
 
-BLOCK = 256          # values of an 8-bit state that share one top
+BLOCK = 256          # values of an 8-bit state that share one top (a value is code * top / 256)
 MAX_WIDTH = 32768    # widest row of block_norm
 
 BlockNormResult = namedtuple("BlockNormResult", "y z post_rstd pre_rstd")
@@ -83,11 +83,11 @@ def _list(op: str, name: str, tensors, sizes=None, dtype=None) -> List:
     _need(not isinstance(tensors, torch.Tensor), TypeError, f"{op}: {name} must be a list of "
                                                             "tensors")
     out = list(tensors)
-    for i, t in enumerate(out):
-        _tensor(op, f"{name}[{i}]", t, dtype or out[0].dtype)
-        _need(t.is_contiguous(), TypeError, f"{op}: {name}[{i}] must be contiguous")
     if out and dtype is None:
-        _tensor(op, f"{name}[0]", out[0])
+        dtype = _tensor(op, f"{name}[0]", out[0]).dtype
+    for i, t in enumerate(out):
+        _tensor(op, f"{name}[{i}]", t, dtype)
+        _need(t.is_contiguous(), TypeError, f"{op}: {name}[{i}] must be contiguous")
     if sizes is not None:
         _need(len(out) == len(sizes), ValueError,
               f"{op}: {name} has {len(out)} tensors, expected {len(sizes)}")
@@ -220,7 +220,7 @@ class Operator:
                      for t, a in zip(self.stream_fn.argtypes, prepared.args))
         args += (ctypes.c_void_p(handle),)
         fn, symbol, index = self.stream_fn, self.symbol, device.index
-        current = torch.cuda.current_device
+        current = torch._C._cuda_getDevice    # current_device() without its checks
 
         def call():
             if current() == index:
@@ -347,8 +347,8 @@ class AdamW(Operator):
               f"{op}: weight_decay has {len(decay)} values, expected {len(params)}")
         beta1, beta2 = (float(b) for b in betas)
         _need(0 <= beta1 < 1 and 0 <= beta2 < 1, ValueError, f"{op}: betas must be in [0, 1)")
-        _need(0 < eps < float("inf") if eight else 0 <= eps < float("inf"), ValueError,
-              f"{op}: eps must be {'above' if eight else 'at least'} zero")
+        least = torch.finfo(torch.float32).tiny if eight else 0.0
+        _need(least <= eps < float("inf"), ValueError, f"{op}: eps must be at least {least}")
         scalars = [t for t in (lr, grad_scale) if t is not None]
         written = params + [t for ts in lists.values() for t in ts] + [step]
         device = _one_device(op, written + grads + scalars)

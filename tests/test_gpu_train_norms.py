@@ -116,6 +116,15 @@ def test_forward_rows(ops, rows, width):
     check_forward(ops, make(rows, width, "bf16", "bf16"), "bf16", "bf16")
 
 
+@pytest.mark.parametrize("width", [104, 249, 257, 264, 1023, 2048, 5001, 8200, 20000])
+@pytest.mark.parametrize("tx,th", TYPES)
+@pytest.mark.parametrize("gate", [None, "token", 6])
+def test_forward_several_rows_a_group(ops, width, tx, th, gate):
+    """More rows than the SMs hold at once, so that row groups walk several."""
+    rows = 6 * (1100 if width < 256 else 500 if width < 1100 else 110)
+    check_forward(ops, make(rows, width, tx, th, gate=gate), tx, th)
+
+
 @pytest.mark.parametrize("gate", [None, "token", "channel", 2, 3])
 @pytest.mark.parametrize("strided", [False, True])
 @pytest.mark.parametrize("width", [96, 257, 2048])
@@ -238,6 +247,14 @@ def test_backward_rows(ops, rows, width):
 def test_backward_gates_and_strides(ops, gate, strided, width):
     check_backward(ops, make(600, width, "f32", "bf16", gate=gate, strided=strided), "f32", "bf16",
                    offset=1.0, a=0.5, b=-2.0)
+
+
+@pytest.mark.parametrize("width", [249, 256, 1536, 4096, 4100, 6144, 8192, 8191])
+@pytest.mark.parametrize("tx,th", [("f32", "f32"), ("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("gate", [None, "token", "channel", 4])
+def test_backward_several_rows_a_group(ops, width, tx, th, gate):
+    check_backward(ops, make(2080 if width == 4096 else 640, width, tx, th, gate=gate), tx, th,
+                   b=0.5, seed=3)
 
 
 @pytest.mark.parametrize("runs", [1500, 750, 300, 1])

@@ -172,7 +172,7 @@ def test_adamw_refuses(ops, change, status):
 
 @pytest.mark.parametrize("change,status", ADAM_BAD + [
     (dict(m_top=None), INVALID), (dict(v_top=_ptrs(FAKE, FAKE + 2)), INVALID),
-    (dict(eps=0.0), INVALID), (dict(eps=1e-60), INVALID)], ids=str)
+    (dict(eps=0.0), INVALID), (dict(eps=1e-60), INVALID), (dict(eps=1e-40), INVALID)], ids=str)
 def test_adamw8_refuses(ops, change, status):
     assert _call(ops["adamw8"], None, **adam_args(True, **change)) == status
 
@@ -194,6 +194,7 @@ ROWS_BAD = [
     (dict(gate_rows=3), INVALID), (dict(gate_rows=0), INVALID), (dict(gate_rows=-2), INVALID),
     (dict(offset=float("nan")), INVALID), (dict(a=float("inf")), INVALID),
     (dict(b=float("nan")), INVALID), (dict(x_stride=-64), INVALID), (dict(x=FAKE + 1), INVALID),
+    (dict(h_stride=1 << 31), INVALID),
     (dict(gate=FAKE + 1), INVALID), (dict(post=FAKE + 1), INVALID)]
 
 
