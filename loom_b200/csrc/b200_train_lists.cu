@@ -206,3 +206,24 @@ extern "C" int loom_train_adamw8(
       weight_decay, param_dtype, grad_dtype, lr, beta1, beta2, eps, grad_scale, step, seed,
       workspace, workspace_size, nullptr));
 }
+
+extern "C" int loom_train_grad_norm_packed(const loom_train_grad_norm_args* a, void* stream) {
+  if (a == nullptr) return LOOM_STATUS_INVALID_ARGUMENT;
+  return loom_train_grad_norm_stream(a->count, a->grads, a->sizes, a->grad_dtype, a->max_norm,
+      a->out, a->workspace, a->workspace_size, stream);
+}
+
+extern "C" int loom_train_adamw_packed(const loom_train_adamw_args* a, void* stream) {
+  if (a == nullptr) return LOOM_STATUS_INVALID_ARGUMENT;
+  return loom_train_adamw_stream(a->count, a->params, a->grads, a->exp_avg, a->exp_avg_sq,
+      a->master, a->sizes, a->weight_decay, a->param_dtype, a->grad_dtype, a->lr, a->beta1,
+      a->beta2, a->eps, a->grad_scale, a->step, a->workspace, a->workspace_size, stream);
+}
+
+extern "C" int loom_train_adamw8_packed(const loom_train_adamw8_args* a, void* stream) {
+  if (a == nullptr) return LOOM_STATUS_INVALID_ARGUMENT;
+  return loom_train_adamw8_stream(a->count, a->params, a->grads, a->exp_avg, a->exp_avg_sq,
+      a->exp_avg_top, a->exp_avg_sq_top, a->master, a->sizes, a->weight_decay, a->param_dtype,
+      a->grad_dtype, a->lr, a->beta1, a->beta2, a->eps, a->grad_scale, a->step, a->seed,
+      a->workspace, a->workspace_size, stream);
+}

@@ -181,3 +181,21 @@ extern "C" int loom_train_block_norm_backward(
       weight_offset, residual_scale, branch_scale, dx, dh, dgate, dpost_weight, dpre_weight,
       workspace, workspace_size, nullptr));
 }
+
+extern "C" int loom_train_block_norm_packed(const loom_train_block_norm_args* a, void* stream) {
+  if (a == nullptr) return LOOM_STATUS_INVALID_ARGUMENT;
+  return loom_train_block_norm_stream(a->x, a->x_stride, a->h, a->h_stride, a->gate,
+      a->gate_stride, a->gate_rows, a->post_weight, a->pre_weight, a->rows, a->width, a->x_dtype,
+      a->h_dtype, a->post_norm, a->pre_norm, a->eps, a->weight_offset, a->residual_scale,
+      a->branch_scale, a->y, a->z, a->post_rstd, a->pre_rstd, stream);
+}
+
+extern "C" int loom_train_block_norm_backward_packed(const loom_train_block_norm_backward_args* a,
+      void* stream) {
+  if (a == nullptr) return LOOM_STATUS_INVALID_ARGUMENT;
+  return loom_train_block_norm_backward_stream(a->y, a->y_stride, a->h, a->h_stride, a->gate,
+      a->gate_stride, a->gate_rows, a->post_weight, a->pre_weight, a->post_rstd, a->pre_rstd,
+      a->dy, a->dy_stride, a->dz, a->dz_stride, a->rows, a->width, a->x_dtype, a->h_dtype,
+      a->post_norm, a->pre_norm, a->weight_offset, a->residual_scale, a->branch_scale, a->dx,
+      a->dh, a->dgate, a->dpost_weight, a->dpre_weight, a->workspace, a->workspace_size, stream);
+}

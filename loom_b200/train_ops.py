@@ -53,6 +53,12 @@ _ARGTYPES = {
 }
 
 
+# the same as the structure of a packed call
+_PACKED = {name: type("Args_" + name, (ctypes.Structure,),
+                      {"_fields_": [(f"a{i}", t) for i, t in enumerate(types)]})
+           for name, types in _ARGTYPES.items()}
+
+
 def _dtype_code(dtype) -> Optional[int]:
     torch = _torch()
     return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(dtype)
@@ -169,6 +175,8 @@ class Operator:
         self.fn.argtypes, self.fn.restype = types, _INT
         self.stream_fn = getattr(lib, meta["stream_symbol"])
         self.stream_fn.argtypes, self.stream_fn.restype = types + [_P], _INT
+        self.packed_fn = getattr(lib, meta["packed_symbol"])
+        self.packed_fn.argtypes, self.packed_fn.restype = [_P, _P], _INT
         self.ws_fn = None
         if meta.get("workspace_symbol"):
             self.ws_fn = getattr(lib, meta["workspace_symbol"])
@@ -216,10 +224,12 @@ class Operator:
         if device.index != torch.cuda.current_device():
             raise ValueError(f"{self.name}: bind with the tensors' device ({device}) current")
         prepared, handle = self._on(stream, kwargs)
-        args = tuple(t(a) if a is not None else None
-                     for t, a in zip(self.stream_fn.argtypes, prepared.args))
-        args += (ctypes.c_void_p(handle),)
-        fn, symbol, index = self.stream_fn, self.symbol, device.index
+        # one structure instead of up to 31 arguments: converting these took half of
+        # a call of one row
+        packed = _PACKED[self.name](*prepared.args)
+        prepared.keep.append(packed)
+        args = (ctypes.c_void_p(ctypes.addressof(packed)), ctypes.c_void_p(handle))
+        fn, symbol, index = self.packed_fn, self.symbol, device.index
         current = torch._C._cuda_getDevice    # current_device() without its checks
 
         def call():

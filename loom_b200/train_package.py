@@ -71,7 +71,8 @@ def _entry_json(entry: str) -> dict:
     text, workspace = ENTRIES[entry]
     sym = symbol_of(entry)
     d = {"entry_name": entry, "module_name": "train", "symbol_name": sym,
-         "stream_symbol": sym + "_stream", "description": text}
+         "stream_symbol": sym + "_stream", "packed_symbol": sym + "_packed",
+         "description": text}
     if workspace:
         d["workspace_symbol"] = sym + "_workspace_size"
     return d

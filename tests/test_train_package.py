@@ -59,13 +59,21 @@ def test_header_declares_what_the_library_exports(ops):
     declared = set(re.findall(r"\b(loom_train_\w+)\(", text))
     listed = set()
     for e in ops.manifest["entries"]:
-        listed |= {e["symbol_name"], e["stream_symbol"]}
+        listed |= {e["symbol_name"], e["stream_symbol"], e["packed_symbol"]}
         if "workspace_symbol" in e:
             listed.add(e["workspace_symbol"])
     assert declared == listed
     for name in declared:
         assert getattr(ops.lib, name) is not None
-    # the loader's argument counts are the header's
+    # the loader's argument counts are the header's, and its structures have the
+    # header's fields' types in the header's order
+    ctype = {"int64_t": ctypes.c_int64, "int": ctypes.c_int, "float": ctypes.c_float,
+             "double": ctypes.c_double, "size_t": ctypes.c_size_t, "uint64_t": ctypes.c_uint64}
+    for e in ops.manifest["entries"]:
+        body = re.search(r"typedef struct %s_args \{(.*?)\}" % e["symbol_name"], text, re.S)
+        fields = [f.strip() for f in body.group(1).split(";") if f.strip()]
+        kinds = [ctypes.c_void_p if "*" in f else ctype[f.split()[0]] for f in fields]
+        assert kinds == [t for _, t in train_ops._PACKED[e["entry_name"]]._fields_]
     for e in ops.manifest["entries"]:
         sig = re.search(re.escape(e["symbol_name"]) + r"\(([^)]*)\);", text).group(1)
         assert len(sig.split(",")) == len(train_ops._ARGTYPES[e["entry_name"]])
@@ -112,9 +120,14 @@ def _i64(*values):
 
 
 def _call(op, stream, **args):
-    """The stream form with these arguments in the declared order."""
+    """The stream form with these arguments in the declared order, and the packed
+    form, which has to say the same."""
     values = [ctypes.addressof(v) if isinstance(v, ctypes.Array) else v for v in args.values()]
-    return op.stream_fn(*values, stream)
+    status = op.stream_fn(*values, stream)
+    packed = train_ops._PACKED[op.name](*values)
+    assert op.packed_fn(ctypes.addressof(packed), stream) == status
+    assert op.packed_fn(None, stream) == INVALID
+    return status
 
 
 def norm_args(**change):
