@@ -239,14 +239,19 @@ __global__ void adamw_begin_kernel(StepValues* __restrict__ out, const float* __
                                    const double beta2, const uint64_t seed) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
-  if (threadIdx.x != 0) return;
   StepValues s = {};
   s.scale = grad_scale != nullptr ? *grad_scale : 1.0f;
   s.skip = !(fabsf(s.scale) < INFINITY);
   const int64_t t = *step + (s.skip ? 0 : 1);
   s.lr = *lr;
-  s.rate = (float)((double)s.lr / (1.0 - pow(beta1, (double)t)));
-  s.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
+  // even lanes raise the one beta, odd lanes the other: the two powers one after
+  // the other were a fifth of a short list's step (8-bit: 4.9 against 6.0 us)
+  const bool second = threadIdx.x & 1;
+  const double rest = 1.0 - pow(second ? beta2 : beta1, (double)t);
+  const float mine = second ? (float)(1.0 / sqrt(rest)) : (float)((double)s.lr / rest);
+  s.rate = __shfl_sync(0xffffffffu, mine, 0);
+  s.root = __shfl_sync(0xffffffffu, mine, 1);
+  if (threadIdx.x != 0) return;
   uint32_t k = mix32((uint32_t)seed ^ kGolden);
   k = mix32(k ^ (uint32_t)(seed >> 32));
   k = mix32(k ^ (uint32_t)t);
