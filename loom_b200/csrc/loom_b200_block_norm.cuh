@@ -824,9 +824,9 @@ inline bool in_phase(const void* p, int64_t stride, int64_t rows, int width) {
 }
 
 // `words`, `fixed`: 16-byte words per thread and group of eight, of a stage and
-// beside the stages; `per`: groups
-// per thread of a staged CTA; `resident`: threads per SM that the kernel's
-// registers allow, about.  `stage`: whether rows come through stages at all.
+// beside the stages; `resident`: threads per SM that the kernel's registers
+// allow, about; `per`: groups per thread of a staged CTA; `stage`: whether rows
+// come through stages at all.
 inline RowPlan row_plan(int width, bool phased, bool stage, int words, int fixed, int resident,
                         int per, bool backward) {
   RowPlan s = {};
@@ -852,7 +852,8 @@ inline RowPlan row_plan(int width, bool phased, bool stage, int words, int fixed
     int ctas = resident / threads;
     if (ctas < 1) ctas = 1;
     // weights beside the stages: see kHold
-    const size_t held = staged && (s.per > 1 || s.most == 1024) ? (size_t)s.per * fixed * 16 * threads : 0;
+    const bool beside = staged && (s.per > 1 || s.most == 1024);
+    const size_t held = beside ? (size_t)s.per * fixed * 16 * threads : 0;
     s.edge = width % 8 != 0 || (staged ? units != (int)s.threads * s.per : !phased || backward);
     if (staged) {
       const size_t bytes = (size_t)s.per * words * 16 * threads;
@@ -883,7 +884,7 @@ inline int64_t step_groups(int64_t groups, int64_t rows, int width, bool phased)
 
 template <class Kern, class... Args>
 inline int launch_rows(Kern kernel, const RowPlan& s, cudaStream_t stream, const Args&... args) {
-  // without the attribute 48 KiB, the kernel's own 256 bytes among them
+  // without the attribute 48 KiB, the kernel's own (under 1 KiB) among them
   if (s.shared > 47 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.shared) !=
           cudaSuccess) {
@@ -921,7 +922,8 @@ inline int with_plan(const RowPlan& s, const F& f) {
     if (s.warp) return f(yes, edge, one, yes, warps);
     if (s.per == 2 && s.most == 256) return f(yes, edge, two, no, quarter);
     if (s.per == 2 && s.most == 512) return f(yes, edge, two, no, half);
-    if constexpr (kBackward) return s.most == 512 ? f(yes, edge, one, no, half) : f(yes, edge, one, no, full);
+    if constexpr (kBackward)
+      return s.most == 512 ? f(yes, edge, one, no, half) : f(yes, edge, one, no, full);
     return f(yes, edge, two, no, full);
   };
   return s.edge ? staged(yes) : staged(no);
@@ -931,7 +933,8 @@ template <class Tx, class Tb>
 int launch_block_norm(const BlockNorm& a, const BlockNormOut& o, cudaStream_t stream) {
   const int w = a.width;
   const bool row_gate = a.gate != nullptr && a.rows_per_gate == 1;
-  const bool phased = in_phase(a.x, a.x_stride, a.rows, w) && in_phase(a.h, a.h_stride, a.rows, w) &&
+  const bool phased = in_phase(a.x, a.x_stride, a.rows, w) &&
+                      in_phase(a.h, a.h_stride, a.rows, w) &&
                       (!row_gate || in_phase(a.gate, a.gate_stride, a.rows, w)) &&
                       in_phase(o.y, w, a.rows, w) && in_phase(o.z, w, a.rows, w);
   // two groups a thread and 512 threads an SM: with one group and twice the
