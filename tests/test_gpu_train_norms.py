@@ -172,6 +172,47 @@ def test_rows_of_zeros_and_of_values_that_are_not_finite(ops):
         assert torch.equal(got.z[row], clean.z[row]) and torch.equal(got.y[row], clean.y[row])
 
 
+def padded(t, pad=8):
+    """The same rows at a stride of `pad` more, NaN between them and behind them."""
+    rows, width = t.shape
+    wide = torch.full((rows, width + pad), float("nan"), device="cuda").to(t.dtype)
+    wide[:, :width] = t
+    return wide[:, :width]
+
+
+@pytest.mark.parametrize("width", [25, 257, 1023, 1536])
+@pytest.mark.parametrize("tx,th", [("bf16", "bf16"), ("f32", "f16")])
+def test_what_lies_between_rows_stays_out(ops, width, tx, th):
+    """Odd widths' groups reach into the row before: rows with NaN between them,
+    and a row of NaN among the others, in both directions."""
+    rows = 2400 if width < 256 else 1700
+    s = make(rows, width, tx, th, gate="token")
+    wide = {k: padded(v) if k in ("x", "h", "gate") else v for k, v in s.items()}
+    want, got = ops["block_norm"](**s), ops["block_norm"](**wide)
+    assert torch.equal(got.y, want.y) and torch.equal(got.z, want.z)
+    rest = {k: v for k, v in s.items() if k != "x"}
+    stats = dict(post_rstd=want.post_rstd, pre_rstd=want.pre_rstd)
+    grads = ops["block_norm_backward"](y=want.y, dy=want.y, dz=want.z, **stats, **rest)
+    rest = {k: v for k, v in wide.items() if k != "x"}
+    again = ops["block_norm_backward"](y=padded(want.y), dy=padded(want.y), dz=padded(want.z),
+                                       **stats, **rest)
+    for a, b in zip(again, grads):
+        assert torch.equal(a, b)
+    bad = 7
+    s["h"][bad] = float("nan")
+    got = ops["block_norm"](**s)
+    others = torch.arange(rows, device="cuda") != bad
+    assert torch.isnan(got.z[bad]).all()
+    assert torch.equal(got.z[others], want.z[others]) and torch.equal(got.y[others],
+                                                                      want.y[others])
+    rest = {k: v for k, v in s.items() if k != "x"}
+    bad_grads = ops["block_norm_backward"](y=got.y, dy=want.y, dz=want.z,
+                                           post_rstd=got.post_rstd, pre_rstd=got.pre_rstd, **rest)
+    assert torch.equal(bad_grads.dx[others], grads.dx[others])
+    assert torch.equal(bad_grads.dh[others], grads.dh[others])
+    assert torch.equal(bad_grads.dgate[others], grads.dgate[others])
+
+
 def test_shapes_and_given_outputs(ops):
     s = make(12, 64, "f32", "bf16", gate=3)
     flat = ops["block_norm"](**s)
