@@ -114,7 +114,7 @@ int loom_train_adamw8_packed(const loom_train_adamw8_args* args, void* stream);
      u = h post_rstd (post_weight + weight_offset), post_rstd = 1 / sqrt(mean(h^2) + eps)   (post_norm 0: u = h)
      y = residual_scale x + branch_scale gate u
      z = y pre_rstd (pre_weight + weight_offset), pre_rstd = 1 / sqrt(mean(y^2) + eps)      (pre_norm 0: no z)
-   x, y are of x_dtype; h, gate, the weights and z of h_dtype (x_dtype, or 16-bit beside a 32-bit x).  rows and strides are below 2^31.  h null: y is x, is not written and may be null.
+   x, y are of x_dtype; h, gate, the weights and z of h_dtype (x_dtype, or 16-bit beside a 32-bit x).  rows and strides are below 2^31.  h null: y is x (residual_scale has no part in it, nor in dx), is not written and may be null.
    gate (or null): gate_rows rows, each for rows / gate_rows consecutive rows.  A null weight is all ones (no offset).  Strides are in elements, outputs contiguous;
    post_rstd and pre_rstd ([rows], for the backward pass) may be null.  Sums are fp32: a row whose sum of squares passes its range has a statistic of 0. */
 int loom_train_block_norm(const void* x, int64_t x_stride, const void* h, int64_t h_stride, const void* gate, int64_t gate_stride, int64_t gate_rows, const void* post_weight, const void* pre_weight, int64_t rows, int64_t width, int x_dtype, int h_dtype, int post_norm, int pre_norm, float eps, float weight_offset, float residual_scale, float branch_scale, void* y, void* z, float* post_rstd, float* pre_rstd);

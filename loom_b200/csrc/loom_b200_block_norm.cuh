@@ -7,8 +7,8 @@
 //   y = residual_scale * x + branch_scale * gate * u
 //   z = y * pre_rstd * (pre_weight + offset),     pre_rstd = 1 / sqrt(mean(y^2) + eps)
 //
-// Each part may be absent: no h (y is x and only z is made), no post norm
-// (u = h), no gate, no weights, no pre norm (only y is made).
+// Each part may be absent: no h (y is x, unscaled, and only z is made), no post
+// norm (u = h), no gate, no weights, no pre norm (only y is made).
 //
 // HBM-bound: about a dozen operations an element on the 8 to 14 bytes that it
 // has to read and write.  So a row is read once and stays in registers between
@@ -983,6 +983,7 @@ int launch_block_norm_grad(const BlockNorm& a0, BlockNormGrad b, int64_t gate_ro
                                   void* dpost_weight, void* dpre_weight, void* workspace,
                                   cudaStream_t stream) {
   BlockNorm a = a0;
+  if (a.h == nullptr) a.residual_scale = 1.0f;  // y is x: nothing scaled it
   const int w = a.width;
   const int64_t rows = a.rows, most = grad_groups_most(rows, w);
   a.rows_per_gate = a.gate != nullptr && rows > 0 ? rows / gate_rows : rows;

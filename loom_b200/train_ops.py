@@ -472,10 +472,11 @@ class BlockNorm(_Norms):
     over the last dimension (at most 32768 wide).  x: the residual stream; h:
     the block's output, of x's type, or 16-bit beside a float32 x; gate: of
     h's type, its rows each serving an equal run of x's rows (as many rows as
-    x, one a sequence, or one for all).  Without h, y is x; a missing weight
-    is all ones; post_norm or pre_norm False leaves that norm out.  Rows may be
-    strided; outputs are contiguous.  `out` (a BlockNormResult) takes the
-    place of new outputs; what is not made is None."""
+    x, one a sequence, or one for all).  Without h, y is x, whatever
+    residual_scale is; a missing weight is all ones; post_norm or pre_norm False
+    leaves that norm out.  Rows may be strided; outputs are contiguous.  `out`
+    (a BlockNormResult) takes the place of new outputs; what is not made is
+    None."""
 
     name = "block_norm"
 

@@ -164,9 +164,10 @@ def block_norm_grads(y, h, gate, post, pre, q, r, dy, dz, *, offset=0.0, a=1.0, 
         d = d + r * (t - n * np.mean(t * n, axis=1, keepdims=True))
         d_abs = d_abs + r * (np.abs(t) + np.abs(n) * np.mean(np.abs(t * n), axis=1, keepdims=True))
         out["dpre_weight"] = ((dz * n).sum(0), np.abs(dz * n).sum(0))
-    out["dx"] = (a * d, np.abs(a) * d_abs)
-    if h is None:
+    if h is None:  # y is x
+        out["dx"] = (d, d_abs)
         return out
+    out["dx"] = (a * d, np.abs(a) * d_abs)
     g = _spread(gate, rows)
     e, e_abs = b * g * d, np.abs(b * g) * d_abs
     if q is None:

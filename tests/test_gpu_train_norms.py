@@ -324,6 +324,17 @@ def test_backward_parts_left_out(ops, form, width):
     check_backward(ops, make(9, width, "bf16", "bf16", **kw), "bf16", "bf16", offset=0.5, **flags)
 
 
+@pytest.mark.parametrize("width", [100, 1023, 1024, 9001])
+@pytest.mark.parametrize("tx,th", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("rows", [9, 700])
+def test_without_h_the_residual_scale_has_no_part(ops, width, tx, th, rows):
+    s = make(rows, width, tx, th, has_h=False)
+    check_forward(ops, s, tx, th, a=0.7, b=3.0, offset=0.5)
+    got = check_backward(ops, s, tx, th, a=0.7, b=3.0, offset=0.5)
+    plain = check_backward(ops, s, tx, th, offset=0.5)
+    assert torch.equal(got.dx, plain.dx) and torch.equal(got.dpre_weight, plain.dpre_weight)
+
+
 def test_backward_of_no_rows(ops):
     s = make(6, 64, "f32", "f32", gate="channel")
     none = {k: (v[:0] if k in ("x", "h") else v) for k, v in s.items()}

@@ -52,6 +52,29 @@ def test_gradients_against_differences(forms):
             assert abs(slope - got[at]) < 1e-7, (key, at, slope, got[at])
 
 
+def test_without_h_the_residual_scale_has_no_part():
+    """y is x then, whatever the scale: its gradient too."""
+    rng = np.random.default_rng(17)
+    x, cy, cz = (rng.normal(size=(3, 6)) for _ in range(3))
+    pre = rng.normal(size=6)
+    kw = dict(offset=0.5, a=0.5)
+
+    def value(x):
+        y, z, *_ = o.block_norm(x, None, None, None, pre, eps=1e-3, **kw)
+        return float((cy * y).sum() + (cz * z).sum())
+
+    y, _, q, r, _ = o.block_norm(x, None, None, None, pre, eps=1e-3, **kw)
+    assert q is None and np.array_equal(y, x)
+    got, _ = o.block_norm_grads(y, None, None, None, pre, q, r, cy, cz, **kw)["dx"]
+    step = 1e-5
+    for at in np.ndindex(x.shape):
+        up, down = x.copy(), x.copy()
+        up[at] += step
+        down[at] -= step
+        # as above: a third derivative of order 10 times step^2, rounding over the step
+        assert abs((value(up) - value(down)) / (2 * step) - got[at]) < 1e-7, at
+
+
 def test_e4m3_values_are_torchs():
     codes = torch.arange(256, dtype=torch.uint8)
     ours = o.e4m3_values()
