@@ -884,10 +884,12 @@ inline int64_t step_groups(int64_t groups, int64_t rows, int width, bool phased)
 
 template <class Kern, class... Args>
 inline int launch_rows(Kern kernel, const RowPlan& s, cudaStream_t stream, const Args&... args) {
-  // without the attribute 48 KiB, the kernel's own (under 1 KiB) among them
+  // Without the attribute 48 KiB, the kernel's own (under 1 KiB) among them.  It
+  // belongs to the function, which serves many widths and host threads: every
+  // call asks for the most that any plan takes, so none lowers another's.
   if (s.shared > 47 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.shared) !=
-          cudaSuccess) {
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)kStageBytes) != cudaSuccess) {
     cudaGetLastError();
     return LOOM_STATUS_CUDA_ERROR;
   }

@@ -475,6 +475,68 @@ def test_a_whole_step_eager_and_replayed(ops, eight):
     assert int(graphed.step) == 6
 
 
+def test_host_threads_with_rows_of_two_widths(ops):
+    """Two threads' launches of one kernel whose rows take different amounts of
+    shared memory: neither may lower what the other has asked for."""
+    import threading
+    sets = [make(1200, width, "bf16", "bf16", gate="token") for width in (2048, 4096)]
+    want, calls, outs = [], [], []
+    for s in sets:
+        out = ops["block_norm"](**s)
+        back = dict(y=out.y, post_rstd=out.post_rstd, pre_rstd=out.pre_rstd, dy=out.y, dz=out.z,
+                    **{k: v for k, v in s.items() if k != "x"})
+        want.append(list(out) + list(ops["block_norm_backward"](**back)))
+        stream = torch.cuda.Stream()
+        f = ops["block_norm"].bind(stream=stream, **s)
+        b = ops["block_norm_backward"].bind(stream=stream, **back)
+        calls.append((f[0], b[0]))
+        outs.append(list(f[1]) + list(b[1]))
+    torch.cuda.synchronize()
+    errors, gate = [], threading.Barrier(2)
+
+    def many(pair):
+        try:
+            gate.wait(timeout=60)
+            for _ in range(1500):
+                for call in pair:
+                    call()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=many, args=(pair,)) for pair in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for got, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
+
+
+def test_a_graph_of_two_widths(ops):
+    """One graph holds launches of one kernel with two amounts of shared memory;
+    eager calls of the smaller one come between its replays."""
+    sets = [make(1200, width, "bf16", "bf16", gate="token") for width in (4096, 2048)]
+    want = [ops["block_norm"](**s) for s in sets]
+    side = torch.cuda.Stream()
+    bound = [ops["block_norm"].bind(stream=side, **s) for s in sets]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for call, _ in bound:
+            call()
+    for _ in range(3):
+        ops["block_norm"](**sets[1])
+        for _, out in bound:
+            out.y.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), w in zip(bound, want):
+            assert torch.equal(out.y, w.y) and torch.equal(out.z, w.z)
+
+
 def test_two_graphs_of_two_bindings_side_by_side(ops):
     """Two graphs, replayed on two streams at once: each binding has a
     workspace of its own."""

@@ -107,6 +107,19 @@ def test_c_programs_run(c_programs):
         assert "train_smoke ok" in proc.stdout
 
 
+def test_row_plans(tmp_path):
+    """Host arithmetic only: no kernel of the program is launched."""
+    if shutil.which("nvcc") is None:
+        pytest.skip("needs nvcc")
+    program = str(tmp_path / "row_plan_check")
+    proc = subprocess.run(["nvcc", "-std=c++17", "-O1", "-gencode", train_package.GENCODE,
+                           f"-I{train_package.CSRC}", os.path.join(HERE, "c", "row_plan_check.cu"),
+                           "-o", program], capture_output=True, text=True)
+    assert proc.returncode == 0, proc.stderr
+    proc = subprocess.run([program], capture_output=True, text=True, timeout=120)
+    assert proc.returncode == 0 and "row plans ok" in proc.stdout, proc.stderr
+
+
 # ---------------------------------------------------------------------------
 # refusals of the C entries
 
