@@ -569,8 +569,7 @@ __device__ __forceinline__ void exchange_and_fold(const typename Op::Acc local,
 // The exchange after a first stage that left this rank's value in `local`
 // (a one-CTA or one-cluster grid); one CTA of 32 threads.
 template <class Op>
-__global__ void peer_exchange_kernel(const typename Op::Acc* __restrict__ local,
-                                     const PeerArgs a) {
+__global__ void peer_exchange_kernel(const typename Op::Acc* local, const PeerArgs a) {
   wait_for_prerequisite_grid();
   exchange_and_fold<Op>(threadIdx.x == 0 ? *local : Op::init(), a);
 }
@@ -580,8 +579,7 @@ __global__ void peer_exchange_kernel(const typename Op::Acc* __restrict__ local,
 // folds theirs.
 template <class Op>
 __global__ void __launch_bounds__(kFinalizeThreads)
-finalize_exchange_kernel(const typename Op::Acc* __restrict__ partials, const int count,
-                         const PeerArgs a) {
+finalize_exchange_kernel(const typename Op::Acc* partials, const int count, const PeerArgs a) {
   wait_for_prerequisite_grid();
   allow_dependent_launch();
   const typename Op::Acc acc = fold_partials<Op>(partials, count);

@@ -472,7 +472,7 @@ reduce_scalar_kernel(typename Op::Acc* __restrict__ partials, const Ptrs<Body::k
 // accumulators, then the CTA tree.  The result is valid in thread 0.
 template <class Op>
 __device__ __forceinline__ typename Op::Acc fold_partials(
-    const typename Op::Acc* __restrict__ partials, const int count) {
+    const typename Op::Acc* partials, const int count) {
   using Acc = typename Op::Acc;
   constexpr int T = kFinalizeThreads;
   constexpr int kLoads = 16;
@@ -495,7 +495,7 @@ __device__ __forceinline__ typename Op::Acc fold_partials(
 // multi-GPU path exchanges it).
 template <class Op>
 __global__ void __launch_bounds__(kFinalizeThreads)
-reduce_finalize_kernel(const typename Op::Acc* __restrict__ partials, const int count,
+reduce_finalize_kernel(const typename Op::Acc* partials, const int count,
                        float* __restrict__ out, typename Op::Acc* __restrict__ partial_out) {
   wait_for_prerequisite_grid();
   allow_dependent_launch();

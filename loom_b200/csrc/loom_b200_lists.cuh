@@ -9,7 +9,8 @@
 // (10 steps at most, uniform over the CTA, in the constant bank).
 //
 // Every kernel is a programmatic dependent launch of the one before it, as in
-// loom_b200_device.cuh.
+// loom_b200_device.cuh.  What it reads may be written while it is already
+// resident, before its wait: no pointer to that promises read-only data.
 #pragma once
 
 #include "loom_b200_launch.cuh"
@@ -82,14 +83,14 @@ list_norm_kernel(const __grid_constant__ NormTable<kCap> t, double* __restrict__
   double acc = 0.0;
   for (uint32_t tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
     const int i = find_tensor(t.first, t.count, tile);
-    const T* __restrict__ g = static_cast<const T*>(t.item[i].g);
+    const T* const g = static_cast<const T*>(t.item[i].g);
     const int64_t n = t.item[i].n;
     // elements before the first 16-byte boundary, and whole vectors after it
     const int64_t lead = (int64_t)((16u - ((uintptr_t)g & 15u)) & 15u) / (int)sizeof(T);
     const int64_t head = lead < n ? lead : n;
     const int64_t nvec = (n - head) / V;
     const int64_t v0 = (int64_t)(tile - t.first[i]) * (kThreads * kNormUnroll);
-    const T* __restrict__ body = g + head;
+    const T* const body = g + head;
     float s[kNormUnroll];
 #pragma unroll
     for (int u = 0; u < kNormUnroll; ++u) s[u] = 0.0f;
@@ -143,8 +144,8 @@ static_assert(sizeof(NormTable<kNormCap>) + kOtherParams <= kParamBytes, "the li
 // where it is no larger, NaN where the sum is not finite (a step given that
 // factor changes nothing).
 __global__ void __launch_bounds__(kFinalizeThreads)
-list_norm_finalize_kernel(const double* __restrict__ partials, const int count,
-                          const float max_norm, float* __restrict__ out) {
+list_norm_finalize_kernel(const double* partials, const int count, const float max_norm,
+                          float* out) {
   wait_for_prerequisite_grid();
   allow_dependent_launch();
   const double sum = fold_partials<SumOp>(partials, count);
@@ -233,10 +234,9 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 
 constexpr uint32_t kGolden = 0x9E3779B9u;
 
-__global__ void adamw_begin_kernel(StepValues* __restrict__ out, const float* __restrict__ lr,
-                                   const float* __restrict__ grad_scale,
-                                   int64_t* __restrict__ step, const double beta1,
-                                   const double beta2, const uint64_t seed) {
+__global__ void adamw_begin_kernel(StepValues* out, const float* lr, const float* grad_scale,
+                                   int64_t* step, const double beta1, const double beta2,
+                                   const uint64_t seed) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
   StepValues s = {};
@@ -266,7 +266,8 @@ inline size_t adamw_workspace_bytes() { return 256 + 256; }
 // reads these 32 bytes, and asking the second level for them each time made
 // its one line the whole step's limit (1026 us for 109M fp32 parameters in
 // tiles of 1024, against 466 for their bytes).  The wait at the kernel's start
-// makes what the kernel before it wrote visible to them.
+// makes what the kernel before it wrote visible to them, as ordinary loads: the
+// pointer carries no __restrict__, which would allow the read-only path.
 __device__ __forceinline__ StepValues step_values(const StepValues* p) {
   const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
   StepValues s;
@@ -327,7 +328,7 @@ __device__ __forceinline__ unsigned phase4(const T* p) {
 // at different places mod 4 elements, single elements are moved instead.
 template <class Tp, class Tg, bool kMaster, int kCap>
 __global__ void __launch_bounds__(kThreads, 6)
-adamw_kernel(const __grid_constant__ AdamTable<kCap> t, const StepValues* __restrict__ values,
+adamw_kernel(const __grid_constant__ AdamTable<kCap> t, const StepValues* values,
              const StepConst c) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();
@@ -549,7 +550,7 @@ struct BlockStage {
 //    slower.
 template <class Tp, class Tg, bool kMaster, int kCap>
 __global__ void __launch_bounds__(kThreads, 3)
-adamw8_kernel(const __grid_constant__ Adam8Table<kCap> t, const StepValues* __restrict__ values,
+adamw8_kernel(const __grid_constant__ Adam8Table<kCap> t, const StepValues* values,
               const StepConst c) {
   allow_dependent_launch();
   wait_for_prerequisite_grid();

@@ -120,6 +120,23 @@ def test_row_plans(tmp_path):
     assert proc.returncode == 0 and "row plans ok" in proc.stdout, proc.stderr
 
 
+def test_dependent_kernels_promise_no_read_only_data():
+    """A kernel that waits for the grid before it is resident while that grid still
+    writes.  A const __restrict__ pointer promises that nobody does, and allows
+    loads through a path that the wait says nothing about."""
+    seen = 0
+    for path in sorted(train_package.CSRC.glob("*.cuh")):
+        parts = re.split(r"(?=__global__)", path.read_text())[1:]
+        for part in parts:
+            kernel = part[:part.index("\n}")]
+            if "wait_for_prerequisite_grid()" not in kernel:
+                continue
+            seen += 1
+            assert not re.search(r"const[\w:<>\s]*\*\s*(const\s+)?__restrict__", kernel), (
+                path.name, kernel[:200])
+    assert seen >= 11
+
+
 # ---------------------------------------------------------------------------
 # refusals of the C entries
 
