@@ -31,7 +31,7 @@ extern "C" {
 #define LOOM_DTYPE_F16 2
 
 /* grad_norm: out[0] = the 2-norm of all values of `count` tensors (sizes[i] values each), out[1] = the factor that brings it down to max_norm (> 0):
-   max_norm / norm where the norm is larger, 1 where it is not, NaN where the sum of squares is not finite (a square beyond the fp32 range counts as infinite). */
+   max_norm / norm where the norm is larger, 1 where it is not, NaN where the sum of squares is not finite (a square beyond the fp32 range counts as infinite; smaller ones add up as they are, however small). */
 size_t loom_train_grad_norm_workspace_size(int64_t count);
 int loom_train_grad_norm(int64_t count, const void* const* grads, const int64_t* sizes, int grad_dtype, float max_norm, float* out, void* workspace, size_t workspace_size);
 int loom_train_grad_norm_stream(int64_t count, const void* const* grads, const int64_t* sizes, int grad_dtype, float max_norm, float* out, void* workspace, size_t workspace_size, void* stream);

@@ -69,11 +69,24 @@ struct NormTable {
   uint32_t tiles;
 };
 
-// Sum of squares of the list, one fp64 partial per CTA.  HBM-bound: one read
-// of each element and two operations on it.  A thread adds its up to 32
-// squares of a tile in fp32 (a fixed tree: no cancellation, at most 5
-// roundings, 3e-7 of the tile's sum) and everything past that in fp64.  A
-// square beyond the fp32 range makes the sum infinite.
+// A square in fp64; one beyond the fp32 range counts as infinite.
+__device__ __forceinline__ double wide_square(float f) {
+  const float q = f * f;
+  return q < INFINITY ? (double)f * (double)f : (double)q;
+}
+
+// Below this a sum of 32 fp32 squares may have lost more than it keeps bits for:
+// squares below 2^-126 are rounded to multiples of 2^-149, so 32 of them are off
+// by 2^-145 at most, 2^-45 of the bound.
+constexpr float kLeastSum = 7.8886090522101181e-31f;      // 2^-100
+
+// Sum of squares of the list, one fp64 partial per CTA.  HBM-bound: one read of
+// each element and two operations on it (411M bf16 values: 120 to 127 us by the
+// box, 105 to 99% of the copy rate).  A thread adds its up to 32 squares of a tile
+// in fp32 (a fixed tree: no cancellation, at most 6 roundings, 3.6e-7 of the
+// tile's sum) and everything past that in fp64.  Where that sum leaves the range in
+// which this holds, on either side, the thread adds the same squares in fp64 (134M
+// fp32 values of 1e-24: 106 us, else 77).
 template <class T, int kCap>
 __global__ void __launch_bounds__(kThreads)
 list_norm_kernel(const __grid_constant__ NormTable<kCap> t, double* __restrict__ partials) {
@@ -91,47 +104,59 @@ list_norm_kernel(const __grid_constant__ NormTable<kCap> t, double* __restrict__
     const int64_t nvec = (n - head) / V;
     const int64_t v0 = (int64_t)(tile - t.first[i]) * (kThreads * kNormUnroll);
     const T* const body = g + head;
-    float s[kNormUnroll];
+    if (v0 + (int)threadIdx.x < nvec) {
+      const uint4* const vecs = reinterpret_cast<const uint4*>(body);
+      uint4 raw[kNormUnroll];
+      if (v0 + kThreads * kNormUnroll <= nvec) {
 #pragma unroll
-    for (int u = 0; u < kNormUnroll; ++u) s[u] = 0.0f;
-    if (v0 + kThreads * kNormUnroll <= nvec) {
-      float f[kNormUnroll][V];
+        for (int u = 0; u < kNormUnroll; ++u)
+          raw[u] = load_word<kStream>(vecs + v0 + u * kThreads + threadIdx.x);
+      } else {
 #pragma unroll
-      for (int u = 0; u < kNormUnroll; ++u)
-        load_vec<V, kStream>(f[u], body + (v0 + u * kThreads + threadIdx.x) * V);
+        for (int u = 0; u < kNormUnroll; ++u) {
+          const int64_t v = v0 + u * kThreads + threadIdx.x;
+          raw[u] = v < nvec ? load_word<kStream>(vecs + v) : make_uint4(0, 0, 0, 0);
+        }
+      }
+      float s[kNormUnroll];
 #pragma unroll
       for (int u = 0; u < kNormUnroll; ++u) {
+        float f[V];
+        widen_word(f, raw[u], T());
 #pragma unroll
         for (int w = V / 2; w > 0; w >>= 1)
 #pragma unroll
           for (int j = 0; j < w; ++j)
-            f[u][j] = w == V / 2 ? fmaf(f[u][j], f[u][j], f[u][j + w] * f[u][j + w])
-                                 : f[u][j] + f[u][j + w];
-        s[u] = f[u][0];
+            f[j] = w == V / 2 ? fmaf(f[j], f[j], f[j + w] * f[j + w]) : f[j] + f[j + w];
+        s[u] = f[0];
       }
-    } else {
+      const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+      if (sum >= kLeastSum && sum < INFINITY) {
+        acc += (double)sum;
+      } else {
+        unsigned any = 0;
 #pragma unroll
-      for (int u = 0; u < kNormUnroll; ++u) {
-        const int64_t v = v0 + u * kThreads + threadIdx.x;
-        if (v < nvec) {
-          float f[V];
-          load_vec<V, kStream>(f, body + v * V);
+        for (int u = 0; u < kNormUnroll; ++u) any |= raw[u].x | raw[u].y | raw[u].z | raw[u].w;
+        if (any & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu)) {  // not zeros alone
+#pragma unroll 1
+          for (int u = 0; u < kNormUnroll; ++u) {
+            float f[V];
+            widen_word(f, raw[0], T());
 #pragma unroll
-          for (int j = 0; j < V; ++j) s[u] = fmaf(f[j], f[j], s[u]);
+            for (int j = 0; j < V; ++j) acc += wide_square(f[j]);
+#pragma unroll
+            for (int k = 1; k < kNormUnroll; ++k) raw[k - 1] = raw[k];
+          }
         }
       }
     }
-    acc += (double)((s[0] + s[1]) + (s[2] + s[3]));
     if (v0 == 0) {  // the tensor's first tile takes its ragged ends
       const int64_t tail0 = head + nvec * V;
       const int r = threadIdx.x;
       int64_t e = -1;
       if (r < head) e = r;
       else if (r >= V && (int64_t)(r - V) < n - tail0) e = tail0 + (r - V);
-      if (e >= 0) {
-        const float f = widen(g[e]);
-        acc += (double)(f * f);
-      }
+      if (e >= 0) acc += wide_square(widen(g[e]));
     }
   }
   acc = block_reduce<SumOp>(acc);

@@ -131,6 +131,20 @@ __device__ __forceinline__ void load_vec(float (&f)[V], const T* p) {
   }
 }
 
+// The elements of a 16-byte word as fp32.
+template <class T>
+__device__ __forceinline__ void widen_word(float (&f)[8], const uint4& w, T) {
+  const unsigned* u = reinterpret_cast<const unsigned*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) widen2(f[2 * i], f[2 * i + 1], u[i], T());
+}
+__device__ __forceinline__ void widen_word(float (&f)[4], const uint4& w, float) {
+  f[0] = __uint_as_float(w.x);
+  f[1] = __uint_as_float(w.y);
+  f[2] = __uint_as_float(w.z);
+  f[3] = __uint_as_float(w.w);
+}
+
 template <int V, Cache kC, class T>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
   constexpr int kBytes = V * (int)sizeof(T);

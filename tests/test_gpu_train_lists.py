@@ -82,6 +82,36 @@ def test_norm_of_values_that_are_not_finite(ops, bad, norm, place):
     assert np.isinf(got[0]) if norm == "inf" else np.isnan(got[0])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e-20, 1e-22, 1e-25, 1e-36, 3e18, 1.2e19])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_norm_of_squares_outside_the_fp32_range(ops, dtype, size, offset):
+    """Squares below the fp32 range, and finite ones whose sum passes it: whole
+    tiles, partial ones and ragged ends."""
+    rng = np.random.default_rng(12)
+    views = [guarded(size * rng.uniform(-1.5, 1.5, size=n), DT[dtype], offset)[0]
+             for n in (1, 5, 4096, 20011, 0, 300)]
+    want, factor = o.norm_and_factor([host(v) for v in views], size)
+    got = ops["grad_norm"](grads=views, max_norm=size).cpu().numpy().astype(np.float64)
+    # as in test_norm_matches
+    assert abs(got[0] - want) <= 4.5 * o.U * want
+    assert abs(got[1] - factor) <= 5.5 * o.U * factor
+
+
+def test_norm_of_zeros_beside_tiny_and_ordinary_values(ops):
+    zeros, tiny_ones = torch.zeros(100000, device="cuda"), torch.zeros(100000, device="cuda")
+    zeros[::2] = -0.0
+    assert ops["grad_norm"](grads=[zeros], max_norm=1.0).cpu().tolist() == [0.0, 1.0]
+    tiny_ones[777] = 1e-30
+    got = ops["grad_norm"](grads=[zeros, tiny_ones], max_norm=1.0).cpu().numpy()
+    want = float(np.float32(1e-30))
+    assert abs(float(got[0]) - want) <= 1.5 * o.U * want and got[1] == 1.0
+    ordinary = torch.ones(100000, device="cuda")
+    got = ops["grad_norm"](grads=[tiny_ones, ordinary], max_norm=1.0).cpu().numpy()
+    want = 1e5 ** 0.5
+    assert abs(float(got[0]) - want) <= 4.5 * o.U * want
+
+
 def test_norm_is_the_same_every_time(ops):
     grads = [torch.randn(n, device="cuda", dtype=torch.bfloat16) for n in (1 << 21, 77, 1 << 19)]
     got = {tuple(ops["grad_norm"](grads=grads, max_norm=1.0).view(torch.int32).tolist())
