@@ -16,6 +16,7 @@ extern "C" {
    - <symbol>_packed is <symbol>_stream with the arguments in one structure, in the same order: for callers to whom each argument of a call costs;
    - a workspace of <symbol>_workspace_size(...) bytes belongs to one call at a time: calls that may overlap on the GPU, two captured graphs among them, each need their own;
    - the return value is one of the status codes of the compiled packages; arguments are checked before anything is launched;
+   - a list has at most 2^40 values in all;
    - arrays of pointers and of sizes are host memory, read during the call only (a captured launch keeps its own copy);
    - tensors that are written may not overlap each other or any that is read. */
 #ifndef LOOM_STATUS_OK

@@ -25,10 +25,15 @@ bool list_ok(int64_t count, const void* const* p, const int64_t* sizes, int byte
   return true;
 }
 
+// At most kListMost values in all, so that the tiles of any launch can be counted
+// in 31 bits: nothing is left to refuse once a step has begun.
 bool sizes_ok(int64_t count, const int64_t* sizes) {
   if (count < 0 || (count > 0 && sizes == nullptr)) return false;
-  for (int64_t i = 0; i < count; ++i)
-    if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 40)) return false;
+  int64_t all = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] < 0 || sizes[i] > loomb::kListMost - all) return false;
+    all += sizes[i];
+  }
   return true;
 }
 

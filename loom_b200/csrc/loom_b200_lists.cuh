@@ -28,6 +28,9 @@ constexpr int kAdamCap = 480;
 constexpr int kAdam8Cap = 360;
 constexpr int kSms = 148;                // of a B200
 
+// Values of a list at most (2^30 tiles of 1024 and one more a tensor).
+constexpr int64_t kListMost = (int64_t)1 << 40;
+
 // What a kernel's parameters may take beside its table.
 constexpr size_t kParamBytes = 32764, kOtherParams = 256;
 
@@ -205,7 +208,6 @@ inline int launch_list_norm_parts(int64_t count, const void* const* grads, const
     for (; i < count && t.count < kCap; ++i) {
       if (sizes[i] == 0) continue;
       const int64_t more = ceil_div(sizes[i], (int64_t)NormTile<T>::value);
-      if (tiles + more > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
       t.item[t.count] = {grads[i], sizes[i]};
       t.first[t.count] = (uint32_t)tiles;
       ++t.count;
@@ -819,7 +821,6 @@ inline int launch_adamw_parts(const AdamLists& l, const StepConst& c, const Step
     for (; i < l.count && t.count < kCap; ++i) {
       if (l.sizes[i] == 0) continue;
       const int64_t more = ceil_div(l.sizes[i], (int64_t)kAdamTile);
-      if (tiles + more > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
       const int k = t.count++;
       t.item[k] = {l.params[i],
                    l.grads[i],
@@ -857,7 +858,6 @@ inline int launch_adamw8_parts(const AdamLists& l, const StepConst& c, const Ste
       if (l.sizes[i] == 0) continue;
       const int64_t blocks = ceil_div(l.sizes[i], (int64_t)kBlock);
       const int64_t more = ceil_div(blocks, per * (kThreads / 32));
-      if (tiles + more > 0x7fffffff) return LOOM_STATUS_INVALID_ARGUMENT;
       const int k = t.count++;
       t.item[k] = {l.params[i],
                    l.grads[i],

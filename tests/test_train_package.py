@@ -220,6 +220,16 @@ def test_adamw8_refuses(ops, change, status):
     assert _call(ops["adamw8"], None, **adam_args(True, **change)) == status
 
 
+@pytest.mark.parametrize("sizes", [(1 << 40, 1), (1 << 40, 1 << 40), (1 << 39, (1 << 39) + 1),
+                                   ((1 << 62), (1 << 62)), (5, (1 << 63) - 1)], ids=str)
+@pytest.mark.parametrize("name", ["grad_norm", "adamw", "adamw8"])
+def test_lists_beyond_their_most_values_are_refused_before_a_launch(ops, name, sizes):
+    """A step that had begun would have counted: the whole list is looked at first."""
+    args = norm_args() if name == "grad_norm" else adam_args(name == "adamw8")
+    args["sizes"] = _i64(*sizes)
+    assert _call(ops[name], None, **args) == INVALID
+
+
 def rows_args(**change):
     a = dict(x=FAKE, x_stride=64, h=FAKE, h_stride=64, gate=FAKE, gate_stride=64, gate_rows=2,
              post=FAKE, pre=FAKE, rows=4, width=64, x_type=1, h_type=1, post_norm=1, pre_norm=1,
