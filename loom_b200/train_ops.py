@@ -132,16 +132,13 @@ def _span(t):
 
 
 def _rows_disjoint(op: str, written, read) -> None:
-    for w in written:
-        if w is None or not w.numel():
-            continue
-        a, b = _span(w)
-        for r in list(read) + [o for o in written if o is not w]:
-            if r is None or not r.numel():
-                continue
-            c, d = _span(r)
+    """No output may overlap another tensor of the call, or be given twice."""
+    outs = [_span(w) for w in written if w is not None and w.numel()]
+    others = [_span(r) for r in read if r is not None and r.numel()]
+    for i, (a, b) in enumerate(outs):
+        for c, d in others + outs[:i]:
             _need(b <= c or d <= a, ValueError,
-                  f"{op}: an output overlaps another tensor of the call")
+                  f"{op}: an output overlaps another tensor of the call (or is given twice)")
 
 
 def _pointers(tensors) -> ctypes.Array:

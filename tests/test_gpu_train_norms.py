@@ -213,6 +213,16 @@ def test_what_lies_between_rows_stays_out(ops, width, tx, th):
     assert torch.equal(bad_grads.dgate[others], grads.dgate[others])
 
 
+def test_an_output_given_twice_is_refused(ops):
+    s = make(12, 64, "f32", "f32")
+    out = ops["block_norm"](**s)
+    with pytest.raises(ValueError):
+        ops["block_norm"](**s, out=out._replace(pre_rstd=out.post_rstd))
+    with pytest.raises(ValueError):
+        ops["block_norm"](**s, out=out._replace(z=out.y))
+    ops["block_norm"](**s, out=out)
+
+
 def test_shapes_and_given_outputs(ops):
     s = make(12, 64, "f32", "bf16", gate=3)
     flat = ops["block_norm"](**s)

@@ -292,6 +292,17 @@ def test_workspace_sizes(ops):
     assert ops["block_norm"].workspace_size() == 0
 
 
+def test_given_outputs_that_overlap_are_refused():
+    import torch
+    buf = torch.zeros(4, 32)
+    a, b, c = buf[0], buf[1], buf[1:3]
+    train_ops._rows_disjoint("op", [a, None, buf[:0]], [b, c, None])
+    for written, read in (([a, a], []), ([a, None, a], []), ([b, c], []), ([c, b], []),
+                          ([a], [a]), ([b], [a, c]), ([buf[:, 8:], a[:9]], [])):
+        with pytest.raises(ValueError):
+            train_ops._rows_disjoint("op", written, read)
+
+
 def test_host_tensors_are_refused(ops):
     import torch
     t = torch.zeros(4)
