@@ -733,7 +733,9 @@ block_norm_grad_kernel(const BlockNorm a, const BlockNormGrad b, const RowPlan p
           s_gate[j] = fma8(own, w, s_gate[j]);
         }
         s_post[j] = s_post[j] + sum;
-        const Group dh = fma8(k[j], post_pull, through * w) * post_rstd;
+        // without the post norm h has no part in it, not even one that is not finite
+        Group dh = through * w;
+        if (post_norm) dh = fma8(k[j], post_pull, dh) * post_rstd;
         if (any[j])
           store_group<kStaged, kEdge>(row_at<Tb>(b.dh, row, width), dh, e[j], width);
       }

@@ -345,6 +345,29 @@ def test_without_h_the_residual_scale_has_no_part(ops, width, tx, th, rows):
     assert torch.equal(got.dx, plain.dx) and torch.equal(got.dpre_weight, plain.dpre_weight)
 
 
+@pytest.mark.parametrize("gate", [None, "token", "channel", 5])
+@pytest.mark.parametrize("width", [100, 1024, 1023])
+@pytest.mark.parametrize("rows", [10, 900])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_without_norms_dh_does_not_hang_on_h(ops, gate, width, rows, bad):
+    """y = a x + b gate h: a value of h that is not finite stays out of dh and dx."""
+    s = make(rows, width, "bf16", "bf16", gate=gate, post=False, pre=False)
+    dy = dev(np.random.default_rng(5).normal(size=(rows, width)), "bf16")
+    call = dict(y=s["x"], dy=dy, gate=s["gate"], post_norm=False, pre_norm=False,
+                residual_scale=0.5, branch_scale=2.0)
+    want = ops["block_norm_backward"](h=s["h"], **call)
+    s["h"][3, 7] = bad
+    got = ops["block_norm_backward"](h=s["h"], **call)
+    assert torch.equal(got.dh, want.dh) and torch.equal(got.dx, want.dx)
+    if gate == "token":  # each gate row's gradient has one row of h
+        assert not torch.isfinite(got.dgate[3, 7])
+        got.dgate[3, 7] = want.dgate[3, 7]
+        assert torch.equal(got.dgate, want.dgate)
+    n = {k: f64(v) for k, v in s.items()}
+    runs = 1.0 if gate is None else np.repeat(n["gate"], rows // n["gate"].shape[0], axis=0)
+    near(got.dh, 2.0 * runs * f64(dy), 3 * o.U * np.abs(2.0 * runs * f64(dy)), "bf16")
+
+
 def test_backward_of_no_rows(ops):
     s = make(6, 64, "f32", "f32", gate="channel")
     none = {k: (v[:0] if k in ("x", "h") else v) for k, v in s.items()}
