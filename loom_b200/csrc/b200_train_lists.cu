@@ -114,7 +114,8 @@ int adamw_impl(const AdamLists& l, int param_dtype, int grad_dtype, const float*
   c.rest1 = (float)(1.0 - beta1);
   c.beta2 = (float)beta2;
   c.rest2 = (float)(1.0 - beta2);
-  c.eps = (float)eps;
+  // an eps below the fp32 range stays above zero: 0 / eps is 0
+  c.eps = eps > 0.0 && (float)eps == 0.0f ? FLT_TRUE_MIN : (float)eps;
   c.zero = -0.0f;
   c.sixteen = 16u;
   StepValues* values = reinterpret_cast<StepValues*>(loomb::workspace_base(workspace));

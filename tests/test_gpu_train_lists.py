@@ -241,6 +241,23 @@ def test_a_factor_that_is_not_finite_skips_the_step(ops, name, factor):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), k
 
 
+@pytest.mark.parametrize("eps", [1e-60, 1e-46, 1e-45, 1e-40])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_adamw_eps_below_the_fp32_range(ops, eps, offset):
+    """A value whose moments are zero does not move, however small eps is."""
+    n = 1000
+    views = {k: guarded(np.full(n, v), torch.float32, offset)[0]
+             for k, v in (("params", 0.5), ("grads", 0.0), ("exp_avg", 0.0), ("exp_avg_sq", 0.0))}
+    views["grads"][::3] = 1e-3
+    ops["adamw"](step=torch.zeros(1, dtype=torch.int64, device="cuda"), lr=1e-2, eps=eps,
+                 betas=(0.9, 0.95), weight_decay=0.0, **{k: [v] for k, v in views.items()})
+    p, _, _, (bp, _, _) = o.adamw(
+        np.full(n, 0.5), host(views["grads"]), np.zeros(n), np.zeros(n), t=1,
+        lr=float(np.float32(1e-2)), beta1=0.9, beta2=0.95, eps=eps, decay=0.0)
+    assert np.all(np.abs(host(views["params"]) - p) <= bp)
+    assert np.all(host(views["params"])[1::3] == 0.5)
+
+
 def test_adamw_on_a_side_stream(ops):
     check_adamw(ops, [70001, 3], "bf16", "bf16", True, stream=torch.cuda.Stream())
 
