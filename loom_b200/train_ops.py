@@ -69,6 +69,11 @@ def _need(cond: bool, exc, text: str) -> None:
         raise exc(text)
 
 
+def _f32(v) -> float:
+    """A number as the C entries get it where they take a float."""
+    return ctypes.c_float(float(v)).value
+
+
 def _tensor(op: str, name: str, t, dtype=None):
     """A CUDA tensor of the given type (or of an operator's three)."""
     torch = _torch()
@@ -281,7 +286,8 @@ class GradNorm(Operator):
         torch = _torch()
         grads = _list(self.name, "grads", grads)
         _need(bool(grads), ValueError, f"{self.name}: no gradients")
-        _need(float(max_norm) > 0, ValueError, f"{self.name}: max_norm must be above zero")
+        _need(_f32(max_norm) > 0, ValueError,
+              f"{self.name}: max_norm must be above zero (as a float32)")
         if out is None:
             out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
         _tensor(self.name, "out", out, torch.float32)
@@ -352,6 +358,8 @@ class AdamW(Operator):
             else [float(weight_decay)] * len(params)
         _need(len(decay) == len(params), ValueError,
               f"{op}: weight_decay has {len(decay)} values, expected {len(params)}")
+        _need(all(abs(w) < float("inf") for w in decay), ValueError,
+              f"{op}: weight_decay must be finite")
         beta1, beta2 = (float(b) for b in betas)
         _need(0 <= beta1 < 1 and 0 <= beta2 < 1, ValueError, f"{op}: betas must be in [0, 1)")
         least = torch.finfo(torch.float32).tiny if eight else 0.0
@@ -411,7 +419,10 @@ def _rows(op: str, name: str, t, width: int, dtype=None):
         _need(v.stride(1) == 1 or width == 1, ValueError,
               f"{op}: the last dimension of {name} must be contiguous")
         rows, stride = v.shape[0], v.stride(0)
-    return rows, (stride if rows > 1 else width)
+    stride = stride if rows > 1 else width
+    _need(rows < 1 << 31 and stride < 1 << 31, ValueError,
+          f"{op}: {name} has {rows} rows at a distance of {stride}; both must be below 2^31")
+    return rows, stride
 
 
 class _Norms(Operator):
@@ -452,8 +463,8 @@ class _Norms(Operator):
 
     def _scales(self, *values):
         for v in values:
-            _need(abs(float(v)) < float("inf"), ValueError,
-                  f"{self.name}: scales and offsets must be finite")
+            _need(abs(_f32(v)) < float("inf"), ValueError,
+                  f"{self.name}: scales and offsets must be finite (as float32)")
         return tuple(float(v) for v in values)
 
 
@@ -484,7 +495,8 @@ class BlockNorm(_Norms):
         op = self.name
         (width, rows, x_stride, h_stride, gate_stride, gate_rows, branch, post_norm,
          pre_norm) = self._common("x", x, h, gate, post_weight, pre_weight, post_norm, pre_norm)
-        _need(0 <= eps < float("inf"), ValueError, f"{op}: eps must be at least zero")
+        _need(0 <= _f32(eps) < float("inf"), ValueError,
+              f"{op}: eps must be at least zero and finite (as a float32)")
         scales = self._scales(weight_offset, residual_scale, branch_scale)
         device = _one_device(op, [x, h, gate, post_weight, pre_weight])
         if out is None:

@@ -450,6 +450,23 @@ def test_refusals(ops):
             ops["adamw8"](**{**eight, **change})
 
 
+def test_numbers_that_are_not_finite_or_beyond_fp32_are_refused(ops):
+    """Before anything runs, as ValueError: the C entries take floats."""
+    t = lambda n=4, d=torch.float32: torch.zeros(n, device="cuda", dtype=d)  # noqa: E731
+    for bad in (1e-50, float("nan"), -1.0):
+        with pytest.raises(ValueError):
+            ops["grad_norm"](grads=[t()], max_norm=bad)
+    assert ops["grad_norm"](grads=[t()], max_norm=1e39).cpu().tolist() == [0.0, 1.0]
+    good = dict(params=[t()], grads=[t()], exp_avg=[t()], exp_avg_sq=[t()],
+                step=t(1, torch.int64), lr=1e-3)
+    for change in (dict(weight_decay=float("nan")), dict(weight_decay=[float("inf")]),
+                   dict(eps=float("inf")), dict(eps=float("nan")),
+                   dict(betas=(0.9, float("nan")))):
+        with pytest.raises(ValueError):
+            ops["adamw"](**{**good, **change})
+    assert int(good["step"]) == 0
+
+
 def test_gradients_may_be_given_twice(ops):
     """What is only read may overlap: one gradient for two tensors."""
     g = torch.randn(100, device="cuda")

@@ -652,3 +652,24 @@ def test_refusals(ops):
                           (dict(dy=out.y.float()), TypeError), (dict(dy=out.y[:3]), ValueError)]:
         with pytest.raises(error):
             g(**{**good, **change})
+
+
+def test_numbers_beyond_fp32_and_rows_beyond_31_bits_are_refused(ops):
+    """Before anything runs, as ValueError: the C entries take floats."""
+    s = make(12, 64, "bf16", "bf16")
+    for change in (dict(eps=1e39), dict(eps=float("inf")), dict(residual_scale=1e39),
+                   dict(branch_scale=-4e38), dict(weight_offset=float("nan"))):
+        with pytest.raises(ValueError):
+            ops["block_norm"](**{**s, **change})
+    # rows that share one place in memory: nothing of this size is allocated
+    many = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(1 << 31, 1)
+    with pytest.raises(ValueError):
+        ops["block_norm"](x=many)
+    with pytest.raises(ValueError):
+        ops["block_norm_backward"](y=many, dz=many, pre_rstd=many)
+    far = torch.empty((1 << 31) + 8, device="cuda", dtype=torch.bfloat16).as_strided(
+        (2, 8), (1 << 31, 1))
+    with pytest.raises(ValueError):
+        ops["block_norm"](x=far)
+    with pytest.raises(ValueError):
+        ops["block_norm"](x=far[:1].expand(2, 8), h=far)
