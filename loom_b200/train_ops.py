@@ -305,9 +305,9 @@ class GradNorm(Operator):
 
 
 class AdamW(Operator):
-    """``adamw(params, grads, exp_avg, exp_avg_sq, step, lr, betas, eps,
-    weight_decay, master=None, grad_scale=None)``: one step of a list of
-    tensors, in place; returns `params`.
+    """``adamw(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
+    eps=1e-8, weight_decay=0, master=None, grad_scale=None)``: one step of a list
+    of tensors, in place; returns `params`.
 
     params, grads: contiguous, each list of one type (float32, bfloat16 or
     float16); exp_avg, exp_avg_sq (and master, the fp32 copies beside 16-bit
@@ -319,8 +319,9 @@ class AdamW(Operator):
 
     name = "adamw"
     state_dtype = "float32"
+    default_betas = (0.9, 0.999)
 
-    def _prepare(self, params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8,
+    def _prepare(self, params, grads, exp_avg, exp_avg_sq, step, lr, betas=None, eps=1e-8,
                  weight_decay=0.0, master=None, grad_scale=None, exp_avg_top=None,
                  exp_avg_sq_top=None, seed=None) -> _Call:
         torch = _torch()
@@ -360,7 +361,7 @@ class AdamW(Operator):
               f"{op}: weight_decay has {len(decay)} values, expected {len(params)}")
         _need(all(abs(w) < float("inf") for w in decay), ValueError,
               f"{op}: weight_decay must be finite")
-        beta1, beta2 = (float(b) for b in betas)
+        beta1, beta2 = (float(b) for b in (self.default_betas if betas is None else betas))
         _need(0 <= beta1 < 1 and 0 <= beta2 < 1, ValueError, f"{op}: betas must be in [0, 1)")
         least = torch.finfo(torch.float32).tiny if eight else 0.0
         _need(least <= eps < float("inf"), ValueError, f"{op}: eps must be at least {least}")
@@ -388,17 +389,18 @@ class AdamW(Operator):
 
 
 class AdamW8(AdamW):
-    """``adamw8(..., exp_avg_top, exp_avg_sq_top, seed)``: the same step with
-    both moments as float8_e4m3fn codes, blocks of 256 values sharing one
-    float32 top (a value is code * top / 256).  New moments are rounded up or
+    """``adamw8(..., betas=(0.9, 0.95), exp_avg_top, exp_avg_sq_top, seed)``: the
+    same step with both moments as float8_e4m3fn codes, blocks of 256 values
+    sharing one float32 top (a value is code * top / 256).  New moments are rounded up or
     down by random bits of `seed`, the step's number and the value's place,
     so that small changes are kept on average; the noise this adds to the
     second moment grows with 1 / (1 - beta2): it is about 12% (one standard
-    deviation) at beta2 = 0.95 and 26% at 0.99, which is as far as 8 bits are
-    meant to be used."""
+    deviation) at beta2 = 0.95, the default here, and 26% at 0.99, which is as
+    far as 8 bits are meant to be used."""
 
     name = "adamw8"
     state_dtype = "float8_e4m3fn"
+    default_betas = (0.9, 0.95)
 
 
 def _rows(op: str, name: str, t, width: int, dtype=None):

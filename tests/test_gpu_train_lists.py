@@ -347,6 +347,20 @@ def test_adamw8_steps(ops, step):
     check_adamw8(ops, [1000, 40], "f32", "bf16", False, step=step)
 
 
+@pytest.mark.parametrize("name,betas", [("adamw", (0.9, 0.999)), ("adamw8", (0.9, 0.95))])
+def test_default_betas(ops, name, betas):
+    """Those of the step's kind: 8-bit moments are not meant for a beta2 of 0.999."""
+    def step(**more):
+        args = eight_state([700], "f32", "f32", False, seed=5)[0] if name == "adamw8" else {
+            k: [v for v, _ in ts] for k, ts in
+            step_lists(np.random.default_rng(9), [700], "f32", "f32", False, 0).items()}
+        ops[name](step=torch.zeros(1, dtype=torch.int64, device="cuda"), lr=1e-2, **args, **more)
+        return [t.view(torch.uint8) for ts in args.values() if isinstance(ts, list) for t in ts]
+
+    for a, b in zip(step(), step(betas=betas)):
+        assert torch.equal(a, b)
+
+
 def test_adamw8_of_a_long_list(ops):
     sizes = [int(n) for n in np.random.default_rng(8).integers(0, 600, size=800)]
     check_adamw8(ops, sizes, "bf16", "bf16", False)
