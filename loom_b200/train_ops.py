@@ -226,6 +226,7 @@ class Operator:
         if device.index != torch.cuda.current_device():
             raise ValueError(f"{self.name}: bind with the tensors' device ({device}) current")
         prepared, handle = self._on(stream, kwargs)
+        self._used_on(handle, stream, prepared)   # should the binding go while a launch runs
         # one structure instead of up to 31 arguments: converting these took half of
         # a call of one row
         packed = _PACKED[self.name](*prepared.args)

@@ -258,6 +258,28 @@ def test_adamw_eps_below_the_fp32_range(ops, eps, offset):
     assert np.all(host(views["params"])[1::3] == 0.5)
 
 
+def test_a_binding_dropped_behind_its_launch(ops):
+    """Inputs of another stream's pool stay as they are until the launch, which
+    waits behind other work of its stream, has read them."""
+    n, side = 1 << 22, torch.cuda.Stream()
+    g = torch.ones(n, device="cuda")
+    call, out = ops["grad_norm"].bind(grads=[g], max_norm=1.0, stream=side)
+    call()   # loading a kernel waits for the device: not in what follows
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1)
+    torch.cuda.synchronize()
+    place = g.data_ptr()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)   # a tenth of a second
+    call()
+    del call, g
+    other = [torch.full((n,), 5.0, device="cuda") for _ in range(4)]
+    early = not side.query()
+    torch.cuda.synchronize()
+    assert early and float(out[0]) == n ** 0.5
+    assert all(t.data_ptr() != place for t in other)
+
+
 def test_adamw_on_a_side_stream(ops):
     check_adamw(ops, [70001, 3], "bf16", "bf16", True, stream=torch.cuda.Stream())
 
