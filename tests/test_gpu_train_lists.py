@@ -112,6 +112,28 @@ def test_norm_of_zeros_beside_tiny_and_ordinary_values(ops):
     assert abs(float(got[0]) - want) <= 4.5 * o.U * want
 
 
+def test_tensors_beyond_31_bits(ops):
+    """A tensor of more than 2^31 elements beside a small one: the norm, and the step
+    of its last elements."""
+    n, tail = (1 << 31) + 70001, 80000
+    g = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    g[-tail:] = torch.randn(tail, device="cuda").to(torch.bfloat16)
+    small = torch.randn(333, device="cuda").to(torch.bfloat16)
+    want, _ = o.norm_and_factor([host(g[-tail:]), host(small)], 1.0)
+    got = ops["grad_norm"](grads=[g, small], max_norm=1.0).cpu().numpy()
+    assert abs(float(got[0]) - want) <= 4.5 * o.U * want
+    p, m, v = (torch.zeros(n, device="cuda", dtype=d)
+               for d in (torch.bfloat16, torch.float32, torch.float32))
+    ops["adamw"](params=[p], grads=[g], exp_avg=[m], exp_avg_sq=[v], lr=1e-2, betas=(0.9, 0.95),
+                 step=torch.zeros(1, dtype=torch.int64, device="cuda"))
+    parts = [torch.zeros(tail, device="cuda", dtype=t.dtype) for t in (p, m, v)]
+    ops["adamw"](params=parts[:1], grads=[g[-tail:].clone()], exp_avg=parts[1:2],
+                 exp_avg_sq=parts[2:], lr=1e-2, betas=(0.9, 0.95),
+                 step=torch.zeros(1, dtype=torch.int64, device="cuda"))
+    for t, part in zip((p, m, v), parts):
+        assert torch.equal(t[-tail:], part) and not t[:-tail].any()
+
+
 def test_norm_is_the_same_every_time(ops):
     grads = [torch.randn(n, device="cuda", dtype=torch.bfloat16) for n in (1 << 21, 77, 1 << 19)]
     got = {tuple(ops["grad_norm"](grads=grads, max_norm=1.0).view(torch.int32).tolist())

@@ -673,3 +673,44 @@ def test_numbers_beyond_fp32_and_rows_beyond_31_bits_are_refused(ops):
         ops["block_norm"](x=far)
     with pytest.raises(ValueError):
         ops["block_norm"](x=far[:1].expand(2, 8), h=far)
+
+
+def test_offsets_beyond_31_bits(ops):
+    """Rows so far apart that elements' places pass 2^31, in both directions."""
+    rows, width, apart = 40, 264, 100_000_000
+    s = make(rows, width, "bf16", "bf16", gate="token")
+    wide = {}
+    for k in ("x", "h", "gate"):
+        buf = torch.empty((rows - 1) * apart + width, device="cuda", dtype=torch.bfloat16)
+        wide[k] = buf.as_strided((rows, width), (apart, 1))
+        wide[k].copy_(s[k])
+    want = ops["block_norm"](**s)
+    got = ops["block_norm"](**{**s, **wide})
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    rest = dict(post_weight=s["post_weight"], pre_weight=s["pre_weight"], dy=want.y, dz=want.z,
+                post_rstd=want.post_rstd, pre_rstd=want.pre_rstd)
+    grads = ops["block_norm_backward"](y=want.y, h=s["h"], gate=s["gate"], **rest)
+    again = ops["block_norm_backward"](y=wide["x"].copy_(want.y), h=wide["h"], gate=wide["gate"],
+                                       **rest)
+    for a, b in zip(again, grads):
+        assert torch.equal(a, b)
+
+
+def test_many_rows_with_outputs_beyond_31_bits(ops):
+    """More than 2^31 elements, contiguous: the last rows are those of a short call."""
+    width, rows = 4096, (1 << 19) + 4096
+    x = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+    s = make(4096, width, "bf16", "bf16", has_h=False)
+    x[-4096:] = s["x"]
+    want = ops["block_norm"](x=s["x"], pre_weight=s["pre_weight"])
+    got = ops["block_norm"](x=x, pre_weight=s["pre_weight"])
+    assert torch.equal(got.z[-4096:], want.z) and not got.z[:-4096].any()
+    assert torch.equal(got.pre_rstd[-4096:], want.pre_rstd)
+    dz = torch.zeros_like(x)
+    dz[-4096:] = want.z
+    grads = ops["block_norm_backward"](y=s["x"], pre_weight=s["pre_weight"], dz=want.z,
+                                       pre_rstd=want.pre_rstd)
+    again = ops["block_norm_backward"](y=x, pre_weight=s["pre_weight"], dz=dz,
+                                       pre_rstd=got.pre_rstd)
+    assert torch.equal(again.dx[-4096:], grads.dx) and not again.dx[:-4096].any()
