@@ -926,9 +926,11 @@ inline int with_plan(const RowPlan& s, const F& f) {
     if (s.warp) return f(yes, edge, one, yes, warps);
     if (s.per == 2 && s.most == 256) return f(yes, edge, two, no, quarter);
     if (s.per == 2 && s.most == 512) return f(yes, edge, two, no, half);
-    if constexpr (kBackward)
+    if constexpr (kBackward) {
       return s.most == 512 ? f(yes, edge, one, no, half) : f(yes, edge, one, no, full);
-    return f(yes, edge, two, no, full);
+    } else {
+      return f(yes, edge, two, no, full);
+    }
   };
   return s.edge ? staged(yes) : staged(no);
 }
@@ -1043,9 +1045,10 @@ int launch_block_norm_grad(const BlockNorm& a0, BlockNormGrad b, int64_t gate_ro
             s, stream, a, b);
       };
       auto by_gate = [&](auto all) {
-        return a.gate == nullptr ? launch(std::integral_constant<int, kNoGate>(), all)
-               : row_gate        ? launch(std::integral_constant<int, kRowGate>(), all)
-                                 : launch(std::integral_constant<int, kRunGate>(), all);
+        if constexpr (decltype(per)::value != 2)  // `two` above leaves run gates out
+          if (run_gate) return launch(std::integral_constant<int, kRunGate>(), all);
+        return row_gate ? launch(std::integral_constant<int, kRowGate>(), all)
+                        : launch(std::integral_constant<int, kNoGate>(), all);
       };
       if constexpr (decltype(staged)::value)
         if (whole) return by_gate(std::true_type());

@@ -120,6 +120,19 @@ def test_row_plans(tmp_path):
     assert proc.returncode == 0 and "row plans ok" in proc.stdout, proc.stderr
 
 
+def test_every_gradient_kernel_can_be_chosen(ops):
+    """Rows of the widest CTA come one group a thread through stages, and so do rows
+    with a gate row per run: the library holds no others with two groups."""
+    if shutil.which("nm") is None:
+        pytest.skip("needs nm")
+    text = subprocess.run(["nm", "-C", ops.path], capture_output=True, text=True).stdout
+    forms = set(re.findall(r"block_norm_grad_kernel<[^,]*, [^,]*, (\w+), \w+, (\d), \w+, (\d+), "
+                           r"\(loomb::Gate\)(\d)", text))
+    assert {("true", "1", "1024", "2"), ("true", "2", "512", "1")} <= forms
+    assert not any(groups == "2" and (threads == "1024" or gate == "2")
+                   for _, groups, threads, gate in forms)
+
+
 def test_dependent_kernels_promise_no_read_only_data():
     """A kernel that waits for the grid before it is resident while that grid still
     writes.  A const __restrict__ pointer promises that nobody does, and allows
