@@ -52,7 +52,8 @@ int loom_train_grad_norm_packed(const loom_train_grad_norm_args* args, void* str
      m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
      p = p (1 - lr weight_decay[i]) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps);  *step = t.
    step and lr are device memory, so that a captured step can be replayed.  master (or null): fp32 copies that the step reads and writes; params then only receive them, rounded.
-   A grad_scale that is not finite skips the step: nothing is changed, *step included. */
+   A grad_scale that is not finite skips the step: nothing is changed, *step included.
+   Every call counts a step: lists that make up one step in several calls (parameters of two types, two learning rates) each need a step of their own. */
 size_t loom_train_adamw_workspace_size(int64_t count);
 int loom_train_adamw(int64_t count, void* const* params, const void* const* grads, float* const* exp_avg, float* const* exp_avg_sq, float* const* master, const int64_t* sizes, const double* weight_decay, int param_dtype, int grad_dtype, const float* lr, double beta1, double beta2, double eps, const float* grad_scale, int64_t* step, void* workspace, size_t workspace_size);
 int loom_train_adamw_stream(int64_t count, void* const* params, const void* const* grads, float* const* exp_avg, float* const* exp_avg_sq, float* const* master, const int64_t* sizes, const double* weight_decay, int param_dtype, int grad_dtype, const float* lr, double beta1, double beta2, double eps, const float* grad_scale, int64_t* step, void* workspace, size_t workspace_size, void* stream);
@@ -117,7 +118,7 @@ int loom_train_adamw8_packed(const loom_train_adamw8_args* args, void* stream);
      z = y pre_rstd (pre_weight + weight_offset), pre_rstd = 1 / sqrt(mean(y^2) + eps)      (pre_norm 0: no z)
    x, y are of x_dtype; h, gate, the weights and z of h_dtype (x_dtype, or 16-bit beside a 32-bit x).  rows and strides are below 2^31.  h null: y is x (residual_scale has no part in it, nor in dx), is not written and may be null.
    gate (or null): gate_rows rows, each for rows / gate_rows consecutive rows.  A null weight is all ones (no offset).  Strides are in elements, outputs contiguous;
-   post_rstd and pre_rstd ([rows], for the backward pass) may be null.  Sums are fp32: a row whose sum of squares passes its range has a statistic of 0. */
+   post_rstd and pre_rstd ([rows], for the backward pass) may be null.  Sums are fp32: a row whose sum of squares passes its range has a statistic of 0, and squares below it count as zero (with eps 0 a row of these has an infinite one). */
 int loom_train_block_norm(const void* x, int64_t x_stride, const void* h, int64_t h_stride, const void* gate, int64_t gate_stride, int64_t gate_rows, const void* post_weight, const void* pre_weight, int64_t rows, int64_t width, int x_dtype, int h_dtype, int post_norm, int pre_norm, float eps, float weight_offset, float residual_scale, float branch_scale, void* y, void* z, float* post_rstd, float* pre_rstd);
 int loom_train_block_norm_stream(const void* x, int64_t x_stride, const void* h, int64_t h_stride, const void* gate, int64_t gate_stride, int64_t gate_rows, const void* post_weight, const void* pre_weight, int64_t rows, int64_t width, int x_dtype, int h_dtype, int post_norm, int pre_norm, float eps, float weight_offset, float residual_scale, float branch_scale, void* y, void* z, float* post_rstd, float* pre_rstd, void* stream);
 typedef struct loom_train_block_norm_args {

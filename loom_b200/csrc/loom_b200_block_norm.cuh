@@ -948,8 +948,13 @@ int launch_block_norm(const BlockNorm& a, const BlockNormOut& o, cudaStream_t st
   // Where there are hardly more rows than row groups, nothing is gained by
   // staging: every row has a CTA or a warp of its own.
   RowPlan s = row_plan(w, phased, true, ForwardStage<Tx, Tb>::words, 0, 512, 2, false);
-  // (1533 rows of 1024, fp32 beside bf16: 6.3 against 7.9 us; of 1040, which leave
-  // threads over, 7.0 against 9.4; but 3000 bf16 rows of 1024 8.9 against 7.3.)
+  // Unstaged against staged, us in a graph, a gate row per row.  Up to here: 1533
+  // rows of 1024, fp32 beside bf16, 6.1 against 7.3; of 1040, which leave threads
+  // over, 6.7 against 9.2; of 1000, 6.5 against 9.0; of 511, 8.4 against 8.6.  Past
+  // it: 3000 bf16 rows of 1024 10.4 against 8.2; of 1023, fp32 beside bf16, 23.3
+  // against 16.6.  The rule is one for all types: it loses up to a quarter with odd
+  // bf16 rows below it (1533 of 1023: 10.4 against 9.3; of 255: 6.5 against 5.3) and
+  // more with fp32 rows beside fp32 past it (3000 of 1024: 12.6 against 20.5).
   if (s.stages == 0 || a.rows <= (w > 1088 ? 1 : s.edge ? 3 : 2) * s.groups) {
     s = row_plan(w, phased, false, 0, 0, 1024, 1, false);
     s.groups = a.rows;

@@ -348,8 +348,8 @@ __device__ __forceinline__ unsigned phase4(const T* p) {
 }
 
 // HBM-bound: 28 bytes and about 14 operations an element with fp32 parameters
-// or with fp32 masters; 109M fp32 parameters take 442 us, 105% of the copy
-// rate.  Four consecutive elements per thread (16 bytes of every fp32 array)
+// or with fp32 masters; 109M fp32 parameters take 442 to 447 us by the box, 105 to
+// 104% of the copy rate.  Four consecutive elements per thread (16 bytes of every fp32 array)
 // and six CTAs per SM: eight or sixteen elements a thread leave fewer warps to
 // cover the loads' latency (455 and 453 us).  Where the arrays of a tensor stand
 // at different places mod 4 elements, single elements are moved instead.
@@ -564,14 +564,18 @@ struct BlockStage {
 // 10 and a sixteenth bytes an element with bf16 parameters and gradients, but
 // bound by issue before HBM: about 60 instructions an element for opening and
 // closing two codes, the random bits and the step.  109M bf16 parameters take
-// 226 us, 74% of the copy rate (one block per warp, 115 instructions an element
-// and loads that nothing overlapped: 587 us).  What it rests on:
+// 226 to 246 us by the box, 74 to 68% of the copy rate (one block per warp, 115
+// instructions an element and loads that nothing overlapped: 587 us); 114M with
+// fp32 masters 359, with fp32 parameters and gradients 396, 78 and 71%.  A tensor
+// with an array that is not aligned takes single elements (101M bf16: 351 against
+// 204).  What it rests on:
 //  * a warp holds a block, eight consecutive values a lane, so a block's
 //    largest is one warp-wide maximum of the values' bit patterns; as unsigned
 //    words these order NaN above infinity above every number, so a block that
 //    holds one that is not finite gets it as its top and reads back as such;
 //  * a warp walks up to 16 consecutive blocks; whole blocks come through shared
-//    memory, three (two for wider types) ahead, at no registers' cost;
+//    memory, three ahead with 16-bit types, two where what the step reads or the
+//    gradients are fp32, one where both are, at no registers' cost;
 //  * packed fp32 instructions for two values at a time;
 //  * three CTAs per SM: bounding the registers for four spills them and is 8%
 //    slower.

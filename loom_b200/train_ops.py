@@ -312,8 +312,9 @@ class AdamW(Operator):
 
     params, grads: contiguous, each list of one type (float32, bfloat16 or
     float16); exp_avg, exp_avg_sq (and master, the fp32 copies beside 16-bit
-    parameters): float32 of the same sizes.  step: one int64, advanced by the
-    call.  lr: one float32, or a number, which a bound call then keeps.
+    parameters): float32 of the same sizes.  step: one int64, advanced by every
+    call: lists that make up one step in several calls (parameters of two
+    types, two learning rates) each need a step of their own.  lr: one float32, or a number, which a bound call then keeps.
     weight_decay: a number, or one per tensor.  grad_scale: one float32 that
     the gradients are multiplied by; where it is not finite the step is
     skipped."""
