@@ -302,6 +302,54 @@ def test_a_binding_dropped_behind_its_launch(ops):
     assert all(t.data_ptr() != place for t in other)
 
 
+@pytest.mark.parametrize("betas", [(0.0, 0.0), (0.0, 0.95), (0.9, 0.0)])
+def test_adamw_without_a_memory(ops, betas):
+    """Betas of zero, with step, rate and factor of no dimensions."""
+    rng = np.random.default_rng(3)
+    views = {k: guarded(np.abs(rng.normal(size=777)), torch.float32, 1)[0]
+             for k in ("params", "grads", "exp_avg", "exp_avg_sq")}
+    old = {k: host(v) for k, v in views.items()}
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")[0]
+    scale = ops["grad_norm"](grads=[views["grads"]], max_norm=1.0)[1]
+    lr = torch.tensor(1e-2, device="cuda")
+    ops["adamw"](step=step, lr=lr, betas=betas, eps=1e-8, weight_decay=0.1, grad_scale=scale,
+                 **{k: [v] for k, v in views.items()})
+    p, m, v, (bp, bm, bv) = o.adamw(old["params"], old["grads"], old["exp_avg"], old["exp_avg_sq"],
+                                    t=1, lr=float(lr), beta1=betas[0], beta2=betas[1], eps=1e-8,
+                                    decay=0.1, scale=float(scale))
+    assert int(step) == 1
+    assert np.all(np.abs(host(views["params"]) - p) <= bp)
+    assert np.all(np.abs(host(views["exp_avg"]) - m) <= bm)
+    assert np.all(np.abs(host(views["exp_avg_sq"]) - v) <= bv)
+
+
+def test_adamw_of_two_types_with_a_step_each(ops):
+    """A step of a model of two parameter types: two calls, one factor, a step tensor
+    for each; the joint norm from the lists' norms."""
+    rng = np.random.default_rng(4)
+    kinds = [("bf16", "bf16", [300, 64]), ("f32", "f32", [33, 5])]
+    lists = [{k: [v for v, _ in ts] for k, ts in step_lists(rng, n, p, g, False, 0).items()}
+             for p, g, n in kinds]
+    norms = [ops["grad_norm"](grads=li["grads"], max_norm=1.0) for li in lists]
+    total = torch.hypot(norms[0][0], norms[1][0])
+    factor = (0.1 / total).clamp(max=1.0)
+    old = [{k: [host(t) for t in ts] for k, ts in li.items()} for li in lists]
+    want, _ = o.norm_and_factor([g for li in old for g in li["grads"]], 1.0)
+    assert abs(float(total) - want) <= 8 * o.U * want
+    steps = [torch.full((1,), 6, dtype=torch.int64, device="cuda") for _ in lists]
+    for li, step in zip(lists, steps):
+        ops["adamw"](step=step, lr=1e-2, betas=(0.9, 0.95), grad_scale=factor, **li)
+    for li, before, step, (kind, _, _) in zip(lists, old, steps, kinds):
+        assert int(step) == 7
+        for i, t in enumerate(li["params"]):
+            p, _, _, (bp, _, _) = o.adamw(
+                before["params"][i], before["grads"][i], before["exp_avg"][i],
+                before["exp_avg_sq"][i], t=7, lr=float(np.float32(1e-2)), decay=0.0,
+                scale=float(factor), **HYPER)
+            slack = half_eps(kind) * (np.abs(p) + bp) + tiny(kind)
+            assert np.all(np.abs(host(t) - p) <= bp + slack)
+
+
 def test_adamw_on_a_side_stream(ops):
     check_adamw(ops, [70001, 3], "bf16", "bf16", True, stream=torch.cuda.Stream())
 

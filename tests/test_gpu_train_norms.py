@@ -714,3 +714,91 @@ def test_many_rows_with_outputs_beyond_31_bits(ops):
     again = ops["block_norm_backward"](y=x, pre_weight=s["pre_weight"], dz=dz,
                                        pre_rstd=got.pre_rstd)
     assert torch.equal(again.dx[-4096:], grads.dx) and not again.dx[:-4096].any()
+
+
+def placed(t, first=1, gap=0):
+    """The same rows `first` elements behind a 16-byte boundary, `gap` apart; NaN
+    around them."""
+    t2 = t if t.dim() == 2 else t[None]
+    rows, width = t2.shape
+    stride = width + gap
+    buf = torch.full((first + rows * stride + 8,), float("nan"), device="cuda").to(t.dtype)
+    v = buf[first:].as_strided((rows, width), (stride, 1))
+    v.copy_(t2)
+    return v if t.dim() == 2 else v[0]
+
+
+@pytest.mark.parametrize("first,gap", [(1, 0), (3, 5), (8, 1), (0, 13)])
+@pytest.mark.parametrize("gate", [None, "token", 3])
+@pytest.mark.parametrize("width", [1, 40, 257, 1024, 4096, 8200])
+@pytest.mark.parametrize("tx,th", [("bf16", "bf16"), ("f32", "f16")])
+def test_rows_at_any_place(ops, width, tx, th, gate, first, gap):
+    """Bases and distances of every alignment, given outputs too, against the same
+    rows at a boundary: within the roundings of sums in another order."""
+    rows = 600 if width < 1000 else 18
+    s = make(rows, width, tx, th, gate=gate)
+    moved = {k: v if v is None else placed(v, first, gap) for k, v in s.items()}
+    check_forward(ops, moved, tx, th, b=0.5)
+    check_backward(ops, moved, tx, th, b=0.5)
+    want = ops["block_norm"](**s, branch_scale=0.5)
+    out = type(want)(*[placed(torch.zeros_like(t), first) for t in want])
+    got = ops["block_norm"](**moved, branch_scale=0.5, out=out)
+    clean = ops["block_norm"](**moved, branch_scale=0.5)
+    for a, b in zip(got, clean):
+        # the outputs' places may choose another kernel: two orders of the fp32 sums
+        near(a, f64(b), 60 * o.U * np.maximum(1.0, np.abs(f64(b))),
+             {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}[a.dtype])
+    n = {k: f64(v) for k, v in s.items()}
+    rng = np.random.default_rng(width)
+    dy, dz = dev(rng.normal(size=(rows, width)), tx), dev(rng.normal(size=(rows, width)), th)
+    call = dict(post_rstd=want.post_rstd, pre_rstd=want.pre_rstd, branch_scale=0.5)
+    got = ops["block_norm_backward"](
+        y=placed(want.y, first, gap), dy=placed(dy, first, gap), dz=placed(dz, first, gap),
+        **{k: v for k, v in moved.items() if k != "x"}, **call)
+    exact = o.block_norm_grads(f64(want.y), n["h"], n["gate"], n["post_weight"], n["pre_weight"],
+                               f64(want.post_rstd), f64(want.pre_rstd), f64(dy), f64(dz), b=0.5)
+    for name, (value, size) in exact.items():   # bounds as in check_backward
+        along = {"dx": 0, "dh": 0, "dgate": 0 if gate is None else rows // s["gate"].shape[0]}
+        near(getattr(got, name), value, (110 + along.get(name, rows)) * o.U * size,
+             tx if name == "dx" else th)
+
+
+@pytest.mark.parametrize("width", [40, 257, 1024])
+def test_rows_that_share_memory(ops, width):
+    """Expanded inputs: every row of x, of the gate and of dy is one row."""
+    s = make(30, width, "f32", "f32", gate="token")
+    for k in ("x", "gate"):
+        s[k] = s[k][:1].expand(30, width)
+    full = {k: v.contiguous() for k, v in s.items()}
+    got, want = ops["block_norm"](**s), ops["block_norm"](**full)
+    check_forward(ops, s, "f32", "f32")
+    check_backward(ops, s, "f32", "f32")
+    near(got.z, f64(want.z), 60 * o.U * np.maximum(1.0, np.abs(f64(want.z))), "f32")
+    dy = s["x"]
+    call = dict(dz=want.z, post_rstd=want.post_rstd, pre_rstd=want.pre_rstd, y=want.y)
+    a = ops["block_norm_backward"](dy=dy, **{k: v for k, v in s.items() if k != "x"}, **call)
+    assert a.dgate.shape == (30, width) and a.dgate.is_contiguous()
+    b = ops["block_norm_backward"](dy=dy.contiguous(),
+                                   **{k: v for k, v in full.items() if k != "x"}, **call)
+    for u, v in zip(a, b):
+        near(u, f64(v), 200 * o.U * np.maximum(8.0, np.abs(f64(v))), "f32")
+
+
+def test_three_dimensions_and_streams_by_handle(ops):
+    """The halves of a projection in three dimensions, on streams given as handles."""
+    both = dev(np.random.default_rng(3).normal(size=(3, 20, 512)), "bf16")
+    x = dev(np.random.default_rng(4).normal(size=(3, 20, 256)), "bf16").requires_grad_()
+    w = torch.ones(256, device="cuda", dtype=torch.bfloat16)
+    a = dict(x=x, h=both[..., :256], gate=both[..., 256:], post_weight=w, pre_weight=w)
+    want = ops["block_norm"](**{k: v.detach().reshape(-1, v.shape[-1]) if v.dim() == 3 else v
+                                for k, v in a.items()})
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (None, 0, side, side.cuda_stream, torch.cuda.current_stream()):
+        got = ops["block_norm"](**a, stream=stream)
+        call, out = ops["block_norm"].bind(**a, stream=stream)
+        call()
+        torch.cuda.synchronize()
+        for t in (got, out):
+            assert t.y.shape == (3, 20, 256) and t.pre_rstd.shape == (60,)
+            assert torch.equal(t.z.view(-1, 256), want.z) and torch.equal(t.y.view(-1, 256), want.y)
