@@ -443,6 +443,8 @@ block_norm_kernel(const BlockNorm a, const BlockNormOut o, const RowPlan plan) {
       copy(row + step * (stages - 1), stage == 0 ? stages - 1 : stage - 1);
       stage = stage == stages - 1 ? 0 : stage + 1;
     }
+    // the statistics by rsqrtf, within 2 ulp: rounded correctly (__frsqrt_rn) they
+    // cost short rows most (65536 x 128 bf16: 32.7 against 29.0 us)
     if (has_h) {
       float rstd = 1.0f;
       if (a.post_norm) {
